@@ -133,6 +133,10 @@ int kernrt_cuda_read_bytes(kernrt_cuda_ctx *ctx, kernrt_buf src, size_t src_byte
                            size_t bytes);
 /* Device address of a buffer (valid until destroy), for zero-copy interop. */
 int kernrt_cuda_device_ptr(kernrt_cuda_ctx *ctx, kernrt_buf buf, void **ptr);
+/* Gives a buffer's memory back once the work already enqueued is done (the
+ * trait frees nothing before the backend goes; a serving process outlives its
+ * requests).  The handle is invalid from then on and is not used again. */
+int kernrt_cuda_free(kernrt_cuda_ctx *ctx, kernrt_buf buf);
 /* Wait for all deferred work. */
 int kernrt_cuda_synchronize(kernrt_cuda_ctx *ctx);
 /* Launch every deferred op (pending embeds, an op held for fusion) onto the
@@ -370,6 +374,109 @@ typedef struct {
 int kernrt_cuda_attention(kernrt_cuda_ctx *ctx, kernrt_buf q, kernrt_buf out, kernrt_buf att, size_t layer,
                           const kernrt_window *windows, size_t n_windows, size_t n_heads, size_t kv_mul,
                           size_t head_size, size_t kv_dim, size_t seq_len);
+
+/* --- Paged key/value cache -----------------------------------------------------
+ * No counterpart in the reference, whose cache is one run of seq_len slots per
+ * layer (mod.rs:169-177) with windows into it.  Here sequences hold pages of
+ * `page_size` positions taken from one pool, so that many sequences of
+ * different lengths share the memory, and sequences forked from one prompt
+ * share its pages.
+ *
+ * A step's calls, in order: kernrt_cuda_pages_step names the sequences that
+ * grow and by how many positions (one each for decoding, a prompt or a chunk
+ * of one for prefill, mixed freely); then for every layer kernrt_cuda_pages_write
+ * stores the new rows of k and v and kernrt_cuda_pages_attention attends the
+ * new rows of q over everything their sequences hold up to and including
+ * their own position.  Rows are packed in the order of the step's sequences.
+ * The step ends with the next pages_step, or with a seq_fork, _copy, _trim,
+ * _close or a pages_compact that moves pages; a layer call after that fails
+ * with KERNRT_E_STATE.
+ *
+ * Pages hold f32 or bf16 (k and v rounded to nearest even).  Layout, all layers
+ * in one allocation: [n_layers][2][n_pages][n_kv_heads][page_size][head_size],
+ * K at 0 and V at 1 of the second axis; zero-filled when made.  head_size is a
+ * multiple of 8 up to 128, page_size 16, 32, 64 or 128, n_heads a multiple of
+ * n_kv_heads.  Query, key, value and output rows are f32.  The attention's sums
+ * are f32 and reordered: it is held to a tolerance, not to the reference's
+ * order, whatever kernrt_cuda_set_exact says.
+ *
+ * Failures of the bookkeeping change nothing: KERNRT_E_STATE when the pool has
+ * too few pages or sequences left, KERNRT_E_INVALID for bad arguments (a closed
+ * sequence, one named twice in a call, a length past max_len). */
+typedef uint64_t kernrt_pages;
+
+/* A cache for at most max_seqs sequences of at most max_len positions over a
+ * pool of n_pages pages. */
+int kernrt_cuda_pages_create(kernrt_cuda_ctx *ctx, int kind, size_t n_layers, size_t n_heads, size_t n_kv_heads,
+                             size_t head_size, size_t page_size, size_t n_pages, size_t max_seqs, size_t max_len,
+                             kernrt_pages *out);
+/* Frees it once the work already enqueued is done. */
+int kernrt_cuda_pages_destroy(kernrt_cuda_ctx *ctx, kernrt_pages pages);
+
+/* The pages' device address (valid until pages_destroy; zero-copy interop, to
+ * save and restore prompts for instance), their shape, and the free pages. */
+typedef struct {
+    void *kv;
+    int kind;
+    uint64_t n_layers, n_pages, n_kv_heads, page_size, head_size;
+    uint64_t available;
+} kernrt_pages_info;
+int kernrt_cuda_pages_ptr(kernrt_cuda_ctx *ctx, kernrt_pages pages, kernrt_pages_info *out);
+
+/* An empty sequence. */
+int kernrt_cuda_seq_open(kernrt_cuda_ctx *ctx, kernrt_pages pages, uint64_t *seq);
+/* n sequences that share the first `length` positions of `seq`, which goes on
+ * unchanged.  No data moves: a sequence that later grows into a page it shares
+ * takes a copy of the page's used rows then (parallel samples, beams, a common
+ * system prompt). */
+int kernrt_cuda_seq_fork(kernrt_cuda_ctx *ctx, kernrt_pages pages, uint64_t seq, size_t length, size_t n,
+                         uint64_t *children);
+/* One sequence with pages of its own, holding a copy of the first `length`
+ * positions of `seq`. */
+int kernrt_cuda_seq_copy(kernrt_cuda_ctx *ctx, kernrt_pages pages, uint64_t seq, size_t length, uint64_t *copy);
+/* Forgets the positions from `length` on (rejected draft tokens, an edited
+ * prompt). */
+int kernrt_cuda_seq_trim(kernrt_cuda_ctx *ctx, kernrt_pages pages, uint64_t seq, size_t length);
+/* Ends n sequences; pages nobody else holds are free again. */
+int kernrt_cuda_seq_close(kernrt_cuda_ctx *ctx, kernrt_pages pages, const uint64_t *seqs, size_t n);
+/* A sequence's length, its number of pages, and the ids of the first
+ * min(capacity, n_pages) of them.  Any output may be NULL (table with
+ * capacity 0). */
+int kernrt_cuda_seq_table(kernrt_cuda_ctx *ctx, kernrt_pages pages, uint64_t seq, size_t *length, int32_t *table,
+                          size_t capacity, size_t *n_pages);
+
+/* Moves the highest pages in use into the lowest free ones (contents and
+ * tables) until the pages in use are the pool's first; *moved (may be NULL)
+ * gets the number moved. */
+int kernrt_cuda_pages_compact(kernrt_cuda_ctx *ctx, kernrt_pages pages, size_t *moved);
+
+/* Sequence seqs[i] grows by rows[i] positions (0: it takes no part), for all i
+ * or, on failure, for none. */
+int kernrt_cuda_pages_step(kernrt_cuda_ctx *ctx, kernrt_pages pages, const uint64_t *seqs, const uint64_t *rows,
+                           size_t n);
+/* The step's rows of k and v, f32 [rows, n_kv_heads * head_size], into `layer`. */
+int kernrt_cuda_pages_write(kernrt_cuda_ctx *ctx, kernrt_pages pages, size_t layer, kernrt_buf k, kernrt_buf v);
+/* out[r, h] = softmax(q[r, h] . K / sqrt(head_size)) V for the step's rows, f32
+ * [rows, n_heads * head_size], over positions 0 .. the row's own; head h reads
+ * kv head h / (n_heads / n_kv_heads).  q != out. */
+int kernrt_cuda_pages_attention(kernrt_cuda_ctx *ctx, kernrt_pages pages, size_t layer, kernrt_buf q, kernrt_buf out);
+
+/* --- Log probabilities of given tokens -------------------------------------------
+ * Beyond the trait, which hands logits to the host.  Per row of logits, f32
+ * [rows, vocab]: logprob = log softmax at the row's target (targets int32 [rows]
+ * in a byte buffer), the entropy in nats, and the `top` largest log
+ * probabilities with their token ids, equal values by ascending id
+ * (top_ids int32 and top_logprobs f32 [rows, top]).  targets and logprob, entropy,
+ * and the top entries (top = 0) may each be left out with 0 handles; top is at
+ * most KERNRT_TOP_MAX and at most vocab.  Outputs are buffers of their own.
+ * Logits of -inf have probability 0.  A row holding NaN or +inf, or only -inf,
+ * has no distribution: its outputs are NaN (its top ids still ordered by value,
+ * NaN first).  A target outside the vocabulary gives NaN and KERNRT_E_DEVICE at
+ * the next barrier. */
+#define KERNRT_TOP_MAX 64
+int kernrt_cuda_logprobs(kernrt_cuda_ctx *ctx, kernrt_buf logits, size_t rows, size_t vocab, kernrt_buf targets,
+                         kernrt_buf logprob, kernrt_buf entropy, size_t top, kernrt_buf top_ids,
+                         kernrt_buf top_logprobs);
 
 /* --- Embedding gather without allocation --------------------------------------
  * No counterpart in the reference: KernRT's backends allocate their own memory.

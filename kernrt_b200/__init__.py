@@ -75,6 +75,13 @@ class StTensor(C.Structure):
                 ("file_offset", C.c_uint64), ("bytes", C.c_uint64)]
 
 
+class PagesInfo(C.Structure):
+    """Mirror of ``kernrt_pages_info``: a paged cache's address, shape and free pages."""
+
+    _fields_ = [("kv", P), ("kind", C.c_int)] + [
+        (n, C.c_uint64) for n in ("n_layers", "n_pages", "n_kv_heads", "page_size", "head_size", "available")]
+
+
 class ChainHostArgs(C.Structure):
     """Mirror of ``kernrt_chain_host_args`` (include/kernrt_cuda.h)."""
 
@@ -141,6 +148,21 @@ SIGNATURES = {
     "kernrt_cuda_prepare_embedding_file": (C.c_int, [P, C.c_char_p, C.c_char_p, C.c_int]),
     "kernrt_cuda_selftest_wait": (C.c_int, [P, C.c_uint64, C.c_int]),
     "kernrt_cuda_set_exact": (C.c_int, [P, C.c_int]),
+    "kernrt_cuda_free": (C.c_int, [P, Buf]),
+    "kernrt_cuda_pages_create": (C.c_int, [P, C.c_int, SZ, SZ, SZ, SZ, SZ, SZ, SZ, SZ, C.POINTER(C.c_uint64)]),
+    "kernrt_cuda_pages_destroy": (C.c_int, [P, C.c_uint64]),
+    "kernrt_cuda_pages_ptr": (C.c_int, [P, C.c_uint64, C.POINTER(PagesInfo)]),
+    "kernrt_cuda_seq_open": (C.c_int, [P, C.c_uint64, C.POINTER(C.c_uint64)]),
+    "kernrt_cuda_seq_fork": (C.c_int, [P, C.c_uint64, C.c_uint64, SZ, SZ, C.POINTER(C.c_uint64)]),
+    "kernrt_cuda_seq_copy": (C.c_int, [P, C.c_uint64, C.c_uint64, SZ, C.POINTER(C.c_uint64)]),
+    "kernrt_cuda_seq_trim": (C.c_int, [P, C.c_uint64, C.c_uint64, SZ]),
+    "kernrt_cuda_seq_close": (C.c_int, [P, C.c_uint64, P, SZ]),
+    "kernrt_cuda_seq_table": (C.c_int, [P, C.c_uint64, C.c_uint64, C.POINTER(SZ), P, SZ, C.POINTER(SZ)]),
+    "kernrt_cuda_pages_compact": (C.c_int, [P, C.c_uint64, C.POINTER(SZ)]),
+    "kernrt_cuda_pages_step": (C.c_int, [P, C.c_uint64, P, P, SZ]),
+    "kernrt_cuda_pages_write": (C.c_int, [P, C.c_uint64, SZ, Buf, Buf]),
+    "kernrt_cuda_pages_attention": (C.c_int, [P, C.c_uint64, SZ, Buf, Buf]),
+    "kernrt_cuda_logprobs": (C.c_int, [P, Buf, SZ, SZ, Buf, Buf, Buf, SZ, Buf, Buf]),
 }
 
 # safetensors dtypes (kernrt_st_tensor.dtype)
@@ -148,6 +170,7 @@ ST_F32, ST_BF16, ST_F16 = 0, 1, 2
 ST_DTYPES = {ST_F32: "F32", ST_BF16: "BF16", ST_F16: "F16"}
 
 NOALLOC_MAX_ROWS = 65536
+TOP_MAX = 64  # KERNRT_TOP_MAX
 
 
 def load() -> C.CDLL:
@@ -315,6 +338,10 @@ class CudaBackend:
         _ok(self._lib.kernrt_cuda_device_ptr(self._ctx, buf, C.byref(p)))
         return p.value or 0
 
+    def free(self, buf: int) -> None:
+        """Gives the buffer's memory back; the handle is not used again."""
+        _ok(self._lib.kernrt_cuda_free(self._ctx, buf))
+
     def synchronize(self) -> None:
         _ok(self._lib.kernrt_cuda_synchronize(self._ctx))
 
@@ -454,6 +481,87 @@ class CudaBackend:
         ws = (Window * max(1, len(windows)))(*[Window(*map(int, w)) for w in windows])
         _ok(self._lib.kernrt_cuda_attention(self._ctx, q, out, att, layer, ws, len(windows), n_heads, kv_mul,
                                             head_size, kv_dim, seq_len))
+
+    # -- the paged key/value cache (beyond the trait) --------------------------------
+    def pages_create(self, kind: int, n_layers: int, n_heads: int, n_kv_heads: int, head_size: int,
+                     page_size: int, n_pages: int, max_seqs: int, max_len: int) -> int:
+        """A pool of pages (kind F32 or BF16) shared by sequences; returns its handle."""
+        h = C.c_uint64()
+        _ok(self._lib.kernrt_cuda_pages_create(self._ctx, kind, n_layers, n_heads, n_kv_heads, head_size, page_size,
+                                               n_pages, max_seqs, max_len, C.byref(h)))
+        return h.value
+
+    def pages_destroy(self, pages: int) -> None:
+        _ok(self._lib.kernrt_cuda_pages_destroy(self._ctx, pages))
+
+    def pages_ptr(self, pages: int) -> PagesInfo:
+        """The pages' device address and shape, and how many are free."""
+        info = PagesInfo()
+        _ok(self._lib.kernrt_cuda_pages_ptr(self._ctx, pages, C.byref(info)))
+        return info
+
+    def seq_open(self, pages: int) -> int:
+        h = C.c_uint64()
+        _ok(self._lib.kernrt_cuda_seq_open(self._ctx, pages, C.byref(h)))
+        return h.value
+
+    def seq_fork(self, pages: int, seq: int, length: int, n: int = 1) -> list[int]:
+        """n sequences sharing the first `length` positions of `seq`."""
+        out = (C.c_uint64 * max(1, n))()
+        _ok(self._lib.kernrt_cuda_seq_fork(self._ctx, pages, seq, length, n, out))
+        return out[:n]
+
+    def seq_copy(self, pages: int, seq: int, length: int) -> int:
+        h = C.c_uint64()
+        _ok(self._lib.kernrt_cuda_seq_copy(self._ctx, pages, seq, length, C.byref(h)))
+        return h.value
+
+    def seq_trim(self, pages: int, seq: int, length: int) -> None:
+        _ok(self._lib.kernrt_cuda_seq_trim(self._ctx, pages, seq, length))
+
+    def seq_close(self, pages: int, seqs) -> None:
+        a = np.ascontiguousarray(seqs, dtype=np.uint64)
+        _ok(self._lib.kernrt_cuda_seq_close(self._ctx, pages, _ptr(a), a.size))
+
+    def seq_length(self, pages: int, seq: int) -> int:
+        n = SZ()
+        _ok(self._lib.kernrt_cuda_seq_table(self._ctx, pages, seq, C.byref(n), None, 0, None))
+        return n.value
+
+    def seq_table(self, pages: int, seq: int) -> np.ndarray:
+        """The ids of the sequence's pages (int32)."""
+        n = SZ()
+        _ok(self._lib.kernrt_cuda_seq_table(self._ctx, pages, seq, None, None, 0, C.byref(n)))
+        out = np.empty(n.value, np.int32)
+        _ok(self._lib.kernrt_cuda_seq_table(self._ctx, pages, seq, None, _ptr(out), out.size, None))
+        return out
+
+    def pages_compact(self, pages: int) -> int:
+        """Moves the pages in use to the front of the pool; returns how many moved."""
+        n = SZ()
+        _ok(self._lib.kernrt_cuda_pages_compact(self._ctx, pages, C.byref(n)))
+        return n.value
+
+    def pages_step(self, pages: int, seqs, rows) -> None:
+        """Sequence seqs[i] grows by rows[i] positions: the step's rows."""
+        s = np.ascontiguousarray(seqs, dtype=np.uint64)
+        r = np.ascontiguousarray(rows, dtype=np.uint64)
+        if s.shape != r.shape:
+            raise ValueError("one row count per sequence")
+        _ok(self._lib.kernrt_cuda_pages_step(self._ctx, pages, _ptr(s), _ptr(r), s.size))
+
+    def pages_write(self, pages: int, layer: int, k: int, v: int) -> None:
+        _ok(self._lib.kernrt_cuda_pages_write(self._ctx, pages, layer, k, v))
+
+    def pages_attention(self, pages: int, layer: int, q: int, out: int) -> None:
+        _ok(self._lib.kernrt_cuda_pages_attention(self._ctx, pages, layer, q, out))
+
+    def logprobs(self, logits: int, rows: int, vocab: int, targets: int = 0, logprob: int = 0, entropy: int = 0,
+                 top: int = 0, top_ids: int = 0, top_logprobs: int = 0) -> None:
+        """kernrt_cuda_logprobs: log probabilities of the targets, entropies and
+        top alternatives of `rows` rows of logits (0 handles leave outputs out)."""
+        _ok(self._lib.kernrt_cuda_logprobs(self._ctx, logits, rows, vocab, targets, logprob, entropy, top, top_ids,
+                                           top_logprobs))
 
     def lfm2_conv_block(self, bcx: int, kernel: int, ring: int, cy: int, rows: int, dim: int,
                         k: int) -> None:

@@ -16,6 +16,8 @@
 // and returned as KERNRT_E_INVALID with a message.
 #include "../../include/kernrt_cuda.h"
 #include "kernels.cuh"
+#include "paged.cuh"
+#include "pages.h"
 #include "safetensors.h"
 
 #include <cuda_runtime.h>
@@ -26,6 +28,7 @@
 #include <fcntl.h>
 #include <unistd.h>
 #include <cstring>
+#include <memory>
 #include <string>
 #include <thread>
 #include <utility>
@@ -90,6 +93,7 @@ public:
         cudaFree(kc_);
         cudaFree(vc_);
         cudaFree(att_scratch_);
+        for (auto &c : caches_) free_cache(c);
         cudaFree(d_err_);
         cudaFree(d_ticket_);
         cudaFree(split_);
@@ -397,6 +401,16 @@ public:
     }
 
     void *device_ptr(kernrt_buf h) { return buf(h).ptr; }
+
+    // Gives a buffer's memory back once the work already queued on it is done;
+    // its handle is not used again.
+    void free_buf(kernrt_buf h) {
+        Buffer &b = buf(h);
+        flush();
+        check(cudaStreamSynchronize(stream_), "synchronize");
+        cudaFree(b.ptr);
+        b = Buffer{};
+    }
 
     // Completes deferred work and surfaces device-reported input errors.
     void barrier() {
@@ -1330,6 +1344,250 @@ public:
         barrier();
     }
 
+    // ---- paged key/value caches (pages.h: the bookkeeping; paged.cu: the device) ----
+    struct PagedCache {
+        std::unique_ptr<PageMap> map;  // null once destroyed
+        PagesView view{};
+        int32_t *table = nullptr;
+        StepSeq *seqs = nullptr;  // the current step's descriptors [max_seqs]
+        bool stepped = false;     // a step is planned and its tables are current
+        size_t n = 0, rows = 0;   // its sequences (those with rows) and rows
+    };
+
+    static void free_cache(PagedCache &c) {
+        cudaFree(c.view.kv);
+        cudaFree(c.table);
+        cudaFree(c.seqs);
+        c = PagedCache{};
+    }
+
+    uint64_t pages_create(int kind, size_t n_layers, size_t n_heads, size_t n_kv_heads, size_t head_size,
+                          size_t page_size, size_t n_pages, size_t max_seqs, size_t max_len) {
+        if (kind != KERNRT_F32 && kind != KERNRT_BF16) fail(KERNRT_E_INVALID, "pages are f32 or bf16");
+        if (n_layers == 0 || n_kv_heads == 0 || n_heads == 0 || n_pages == 0 || max_seqs == 0 || max_len == 0)
+            fail(KERNRT_E_INVALID, "empty page cache");
+        if (n_heads % n_kv_heads != 0) fail(KERNRT_E_INVALID, "n_heads is not a multiple of n_kv_heads");
+        if (head_size == 0 || head_size % 8 != 0 || head_size > 128)
+            fail(KERNRT_E_INVALID, "head_size must be a multiple of 8 up to 128");
+        if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128)
+            fail(KERNRT_E_INVALID, "page_size must be 16, 32, 64 or 128");
+        const size_t big = (size_t)INT32_MAX;
+        if (n_layers > 65535 || n_heads > 65535 || max_seqs > 65535 || n_pages > big / 4 || max_len > big / 4)
+            fail(KERNRT_E_INVALID, "page cache too large");
+        // rows of head_size elements, addressed by a signed 32-bit coordinate
+        if (n_layers * 2 * n_kv_heads * page_size > big / n_pages) fail(KERNRT_E_INVALID, "page cache too large");
+        const size_t max_pages = (max_len + page_size - 1) / page_size;
+        if (max_pages > big / max_seqs) fail(KERNRT_E_INVALID, "page tables too large");
+        flush();
+        PagedCache c;
+        c.map = std::make_unique<PageMap>(n_pages, page_size, max_seqs, max_len);
+        const size_t bytes = n_layers * 2 * n_pages * n_kv_heads * page_size * head_size * (kind == KERNRT_F32 ? 4 : 2);
+        try {
+            check(cudaMalloc(&c.view.kv, bytes), "cudaMalloc(pages)");
+            check(cudaMalloc(&c.table, max_seqs * max_pages * sizeof(int32_t)), "cudaMalloc(page tables)");
+            check(cudaMalloc(&c.seqs, max_seqs * sizeof(StepSeq)), "cudaMalloc(step)");
+            check(cudaMemsetAsync(c.view.kv, 0, bytes, stream_), "cudaMemset");
+            check(cudaMemsetAsync(c.table, 0, max_seqs * max_pages * sizeof(int32_t), stream_), "cudaMemset");
+        } catch (...) {
+            free_cache(c);
+            throw;
+        }
+        PagesView &v = c.view;
+        v.f32 = kind == KERNRT_F32;
+        v.n_layers = (int)n_layers;
+        v.n_pages = (int)n_pages;
+        v.kv_heads = (int)n_kv_heads;
+        v.heads = (int)n_heads;
+        v.group = (int)(n_heads / n_kv_heads);
+        v.head = (int)head_size;
+        v.page_shift = page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7;
+        v.table = c.table;
+        v.max_pages = (int)max_pages;
+        caches_.push_back(std::move(c));
+        return (uint64_t)caches_.size();  // handle = index + 1
+    }
+
+    PagedCache &cache(uint64_t h) {
+        if (h == 0 || h > caches_.size() || !caches_[h - 1].map)
+            fail(KERNRT_E_INVALID, "invalid page cache handle " + std::to_string(h));
+        return caches_[h - 1];
+    }
+
+    void pages_destroy(uint64_t h) {
+        PagedCache &c = cache(h);
+        flush();
+        check(cudaStreamSynchronize(stream_), "synchronize");
+        free_cache(c);
+    }
+
+    // The bookkeeping's refusals as this library's errors.
+    template <class F>
+    static auto paging(F &&fn) {
+        try {
+            return fn();
+        } catch (const PageError &e) {
+            fail(e.exhausted ? KERNRT_E_STATE : KERNRT_E_INVALID, e.msg);
+        }
+    }
+
+    void copy_pages(PagedCache &c, const std::vector<PageCopy> &copies) {
+        static_assert(sizeof(PageCopy) == sizeof(CopyItem), "one layout");
+        if (copies.empty()) return;
+        const auto *d = static_cast<const CopyItem *>(stage(copies.data(), copies.size() * sizeof(CopyItem)));
+        launch_or_fail(launch_pages_copy(c.view, d, (int)copies.size(), stream_), "pages_copy");
+    }
+
+    void seq_fork(uint64_t h, uint64_t seq, size_t length, size_t n, uint64_t *out) {
+        PagedCache &c = cache(h);
+        if (n && !out) fail(KERNRT_E_INVALID, "null output pointer");
+        const std::vector<uint64_t> got = paging([&] { return c.map->fork(seq, length, n); });
+        c.stepped = false;
+        std::copy(got.begin(), got.end(), out);
+    }
+
+    uint64_t seq_copy(uint64_t h, uint64_t seq, size_t length) {
+        PagedCache &c = cache(h);
+        flush();
+        std::vector<PageCopy> copies;
+        const uint64_t got = paging([&] { return c.map->copy(seq, length, &copies); });
+        c.stepped = false;
+        copy_pages(c, copies);
+        return got;
+    }
+
+    void seq_trim(uint64_t h, uint64_t seq, size_t length) {
+        PagedCache &c = cache(h);
+        paging([&] { c.map->trim(seq, length); });
+        c.stepped = false;
+    }
+
+    void seq_close(uint64_t h, const uint64_t *seqs, size_t n) {
+        PagedCache &c = cache(h);
+        if (n && !seqs) fail(KERNRT_E_INVALID, "null sequences");
+        paging([&] { c.map->close(seqs, n); });
+        c.stepped = false;
+    }
+
+    size_t pages_compact(uint64_t h) {
+        PagedCache &c = cache(h);
+        flush();
+        const std::vector<PageCopy> moves = c.map->compact();
+        if (!moves.empty()) c.stepped = false;
+        copy_pages(c, moves);
+        return moves.size();
+    }
+
+    // The next step of the sequences: each grows by its rows, its table goes
+    // up to date on the device, and the step's descriptors are laid down for
+    // every layer's pages_write and pages_attention.
+    void pages_step(uint64_t h, const uint64_t *seqs, const uint64_t *rows, size_t n) {
+        PagedCache &c = cache(h);
+        if (n && (!seqs || !rows)) fail(KERNRT_E_INVALID, "null sequences or rows");
+        if (n > c.map->max_seqs()) fail(KERNRT_E_INVALID, "more sequences in a step than the cache holds");
+        size_t total = 0;
+        for (size_t i = 0; i < n; ++i) {
+            if (rows[i] > (uint64_t)INT32_MAX) fail(KERNRT_E_INVALID, "too many rows in one step");
+            total += (size_t)rows[i];
+        }
+        fits_int(total * 2, "pages_step");
+        flush();
+        std::vector<PageCopy> copies;
+        paging([&] { c.map->extend(seqs, rows, n, &copies); });
+        c.stepped = false;
+        copy_pages(c, copies);
+        std::vector<StepSeq> desc;
+        std::vector<int32_t> delta;
+        size_t row0 = 0;
+        for (size_t i = 0; i < n; ++i) {
+            if (rows[i] == 0) continue;
+            const size_t slot = c.map->slot(seqs[i]);
+            const PageMap::Seq &q = c.map->at(slot);
+            StepSeq d{};
+            d.slot = (int32_t)slot;
+            d.ctx = (int32_t)(q.len - rows[i]);
+            d.rows = (int32_t)rows[i];
+            d.row0 = (int32_t)row0;
+            d.dirty = (int32_t)q.dirty;
+            d.n_dirty = (int32_t)(q.pages.size() - q.dirty);
+            d.delta = (int32_t)delta.size();
+            delta.insert(delta.end(), q.pages.begin() + (long)q.dirty, q.pages.end());
+            desc.push_back(d);
+            row0 += (size_t)rows[i];
+        }
+        c.n = desc.size();
+        c.rows = row0;
+        if (c.n) {
+            std::vector<char> block(desc.size() * sizeof(StepSeq) + delta.size() * sizeof(int32_t));
+            std::memcpy(block.data(), desc.data(), desc.size() * sizeof(StepSeq));
+            if (!delta.empty())
+                std::memcpy(block.data() + desc.size() * sizeof(StepSeq), delta.data(), delta.size() * sizeof(int32_t));
+            const auto *d = static_cast<const StepSeq *>(stage(block.data(), block.size()));
+            launch_or_fail(launch_pages_step(d, (int)c.n, c.seqs, c.table, c.view.max_pages, stream_), "pages_step");
+            for (const StepSeq &d2 : desc) c.map->at((size_t)d2.slot).dirty = c.map->at((size_t)d2.slot).pages.size();
+        }
+        c.stepped = true;
+    }
+
+    PagedCache &stepped_cache(uint64_t h, size_t layer) {
+        PagedCache &c = cache(h);
+        if (!c.stepped) fail(KERNRT_E_STATE, "pages_step() runs before the step's layers");
+        if (layer >= (size_t)c.view.n_layers) fail(KERNRT_E_INVALID, "layer out of range of the page cache");
+        return c;
+    }
+
+    void pages_write(uint64_t h, size_t layer, kernrt_buf k, kernrt_buf v) {
+        PagedCache &c = stepped_cache(h, layer);
+        Buffer &kb = buf(k), &vb = buf(v);
+        const size_t width = (size_t)c.view.kv_heads * c.view.head;
+        span(kb, 0, c.rows * width, "pages_write k");
+        span(vb, 0, c.rows * width, "pages_write v");
+        flush();
+        launch_or_fail(launch_pages_write(c.view, (int)layer, c.seqs, (int)c.n, (int)c.rows, f(kb), f(vb), stream_),
+                       "pages_write");
+    }
+
+    void pages_attention(uint64_t h, size_t layer, kernrt_buf q, kernrt_buf out) {
+        PagedCache &c = stepped_cache(h, layer);
+        distinct(q, out);
+        Buffer &qb = buf(q), &ob = buf(out);
+        const size_t width = (size_t)c.view.heads * c.view.head;
+        span(qb, 0, c.rows * width, "pages_attention q");
+        span(ob, 0, c.rows * width, "pages_attention out");
+        flush();
+        launch_or_fail(launch_pages_attention_rows(c.view, (int)layer, c.seqs, (int)c.n, (int)c.rows, f(qb), f(ob),
+                                                   stream_),
+                       "pages_attention");
+    }
+
+    // ---- log probabilities of given tokens (logprobs.cu) ------------------------
+    void logprobs(kernrt_buf logits, size_t rows, size_t vocab, kernrt_buf targets, kernrt_buf logprob,
+                  kernrt_buf entropy, size_t top, kernrt_buf top_ids, kernrt_buf top_logprobs) {
+        if (vocab == 0 || vocab > (size_t)INT32_MAX / 2) fail(KERNRT_E_INVALID, "logprobs: bad vocabulary size");
+        if (top > KERNRT_TOP_MAX || top > vocab) fail(KERNRT_E_INVALID, "logprobs: too many top entries");
+        if ((targets != 0) != (logprob != 0)) fail(KERNRT_E_INVALID, "logprobs: targets and logprob come together");
+        if (top ? !top_ids || !top_logprobs : top_ids || top_logprobs)
+            fail(KERNRT_E_INVALID, "logprobs: top entries need their ids and log probabilities");
+        if (rows > (size_t)INT32_MAX / 64) fail(KERNRT_E_INVALID, "logprobs: too many rows");
+        Buffer &xb = buf(logits);
+        if (rows > xb.bytes / 4 / vocab) fail(KERNRT_E_INVALID, "logprobs: logits buffer too small");
+        const kernrt_buf outs[4] = {logprob, entropy, top_ids, top_logprobs};
+        const size_t lens[4] = {rows, rows, rows * top, rows * top};
+        for (int i = 0; i < 4; ++i) {
+            if (!outs[i]) continue;
+            distinct(outs[i], logits);
+            if (outs[i] == targets) fail(KERNRT_E_INVALID, "buffers must be distinct");
+            for (int j = 0; j < i; ++j) distinct(outs[i], outs[j]);
+            span(buf(outs[i]), 0, lens[i], "logprobs output");
+        }
+        if (targets) span(buf(targets), 0, rows, "logprobs targets");
+        flush();
+        auto ints = [&](kernrt_buf h) { return h ? reinterpret_cast<int32_t *>(buf(h).ptr) : nullptr; };
+        auto floats = [&](kernrt_buf h) { return h ? f(buf(h)) : nullptr; };
+        launch_or_fail(launch_logprobs(f(xb), (int)rows, (int)vocab, ints(targets), floats(logprob), floats(entropy),
+                                       (int)top, ints(top_ids), floats(top_logprobs), d_err_, stream_),
+                       "logprobs");
+    }
+
     // ---- stage timing: CUDA events around each kernel of a chain launch --------
     void stage_timing(bool on) {
         flush();
@@ -1489,7 +1747,8 @@ private:
     };
 
     Buffer &buf(kernrt_buf h) {
-        if (h == 0 || h > bufs_.size()) fail(KERNRT_E_INVALID, "invalid buffer handle " + std::to_string(h));
+        if (h == 0 || h > bufs_.size() || !bufs_[h - 1].ptr)
+            fail(KERNRT_E_INVALID, "invalid buffer handle " + std::to_string(h));
         return bufs_[h - 1];
     }
     static float *f(Buffer &b) { return reinterpret_cast<float *>(b.ptr); }
@@ -1725,6 +1984,7 @@ private:
     std::vector<RopeTable> ropes_;
     std::vector<Pending> pending_;
     std::vector<DevMatrix> mats_;
+    std::vector<PagedCache> caches_;
     float *kc_ = nullptr, *vc_ = nullptr;
     float *att_scratch_ = nullptr;
     size_t att_scratch_bytes_ = 0;
@@ -2110,6 +2370,103 @@ int kernrt_cuda_attention(kernrt_cuda_ctx *ctx, kernrt_buf q, kernrt_buf out, ke
                           size_t head_size, size_t kv_dim, size_t seq_len) {
     return guard(ctx, [&](krt::Backend &b) {
         b.attention(q, out, att, layer, windows, n_windows, n_heads, kv_mul, head_size, kv_dim, seq_len);
+    });
+}
+
+int kernrt_cuda_free(kernrt_cuda_ctx *ctx, kernrt_buf buf) {
+    return guard(ctx, [&](krt::Backend &b) { b.free_buf(buf); });
+}
+
+int kernrt_cuda_pages_create(kernrt_cuda_ctx *ctx, int kind, size_t n_layers, size_t n_heads, size_t n_kv_heads,
+                             size_t head_size, size_t page_size, size_t n_pages, size_t max_seqs, size_t max_len,
+                             kernrt_pages *out) {
+    if (!out) {
+        g_last_error = "null output pointer";
+        return KERNRT_E_INVALID;
+    }
+    return guard(ctx, [&](krt::Backend &b) {
+        *out = b.pages_create(kind, n_layers, n_heads, n_kv_heads, head_size, page_size, n_pages, max_seqs, max_len);
+    });
+}
+
+int kernrt_cuda_pages_destroy(kernrt_cuda_ctx *ctx, kernrt_pages pages) {
+    return guard(ctx, [&](krt::Backend &b) { b.pages_destroy(pages); });
+}
+
+int kernrt_cuda_pages_ptr(kernrt_cuda_ctx *ctx, kernrt_pages pages, kernrt_pages_info *out) {
+    return guard(ctx, [&](krt::Backend &b) {
+        if (!out) krt::fail(KERNRT_E_INVALID, "null output pointer");
+        const krt::PagesView &v = b.cache(pages).view;
+        *out = {v.kv, v.f32 ? KERNRT_F32 : KERNRT_BF16, (uint64_t)v.n_layers, (uint64_t)v.n_pages,
+                (uint64_t)v.kv_heads, (uint64_t)1 << v.page_shift, (uint64_t)v.head,
+                (uint64_t)b.cache(pages).map->available()};
+    });
+}
+
+int kernrt_cuda_seq_open(kernrt_cuda_ctx *ctx, kernrt_pages pages, uint64_t *seq) {
+    return guard(ctx, [&](krt::Backend &b) {
+        if (!seq) krt::fail(KERNRT_E_INVALID, "null output pointer");
+        *seq = krt::Backend::paging([&] { return b.cache(pages).map->open(); });
+    });
+}
+
+int kernrt_cuda_seq_fork(kernrt_cuda_ctx *ctx, kernrt_pages pages, uint64_t seq, size_t length, size_t n,
+                         uint64_t *children) {
+    return guard(ctx, [&](krt::Backend &b) { b.seq_fork(pages, seq, length, n, children); });
+}
+
+int kernrt_cuda_seq_copy(kernrt_cuda_ctx *ctx, kernrt_pages pages, uint64_t seq, size_t length, uint64_t *copy) {
+    return guard(ctx, [&](krt::Backend &b) {
+        if (!copy) krt::fail(KERNRT_E_INVALID, "null output pointer");
+        *copy = b.seq_copy(pages, seq, length);
+    });
+}
+
+int kernrt_cuda_seq_trim(kernrt_cuda_ctx *ctx, kernrt_pages pages, uint64_t seq, size_t length) {
+    return guard(ctx, [&](krt::Backend &b) { b.seq_trim(pages, seq, length); });
+}
+
+int kernrt_cuda_seq_close(kernrt_cuda_ctx *ctx, kernrt_pages pages, const uint64_t *seqs, size_t n) {
+    return guard(ctx, [&](krt::Backend &b) { b.seq_close(pages, seqs, n); });
+}
+
+int kernrt_cuda_seq_table(kernrt_cuda_ctx *ctx, kernrt_pages pages, uint64_t seq, size_t *length, int32_t *table,
+                          size_t capacity, size_t *n_pages) {
+    return guard(ctx, [&](krt::Backend &b) {
+        const krt::PageMap &m = *b.cache(pages).map;
+        const krt::PageMap::Seq &q = m.at(krt::Backend::paging([&] { return m.slot(seq); }));
+        if (length) *length = q.len;
+        if (n_pages) *n_pages = q.pages.size();
+        if (capacity && !table) krt::fail(KERNRT_E_INVALID, "null table");
+        std::copy(q.pages.begin(), q.pages.begin() + (long)std::min(capacity, q.pages.size()), table);
+    });
+}
+
+int kernrt_cuda_pages_compact(kernrt_cuda_ctx *ctx, kernrt_pages pages, size_t *moved) {
+    return guard(ctx, [&](krt::Backend &b) {
+        const size_t n = b.pages_compact(pages);
+        if (moved) *moved = n;
+    });
+}
+
+int kernrt_cuda_pages_step(kernrt_cuda_ctx *ctx, kernrt_pages pages, const uint64_t *seqs, const uint64_t *rows,
+                           size_t n) {
+    return guard(ctx, [&](krt::Backend &b) { b.pages_step(pages, seqs, rows, n); });
+}
+
+int kernrt_cuda_pages_write(kernrt_cuda_ctx *ctx, kernrt_pages pages, size_t layer, kernrt_buf k, kernrt_buf v) {
+    return guard(ctx, [&](krt::Backend &b) { b.pages_write(pages, layer, k, v); });
+}
+
+int kernrt_cuda_pages_attention(kernrt_cuda_ctx *ctx, kernrt_pages pages, size_t layer, kernrt_buf q, kernrt_buf out) {
+    return guard(ctx, [&](krt::Backend &b) { b.pages_attention(pages, layer, q, out); });
+}
+
+int kernrt_cuda_logprobs(kernrt_cuda_ctx *ctx, kernrt_buf logits, size_t rows, size_t vocab, kernrt_buf targets,
+                         kernrt_buf logprob, kernrt_buf entropy, size_t top, kernrt_buf top_ids,
+                         kernrt_buf top_logprobs) {
+    return guard(ctx, [&](krt::Backend &b) {
+        b.logprobs(logits, rows, vocab, targets, logprob, entropy, top, top_ids, top_logprobs);
     });
 }
 

@@ -1,0 +1,53 @@
+// Launch interface of the paged key/value cache's kernels (paged.cu) and of
+// the token log probabilities (logprobs.cu).  All pointers are device
+// pointers; all launches are asynchronous on the given stream.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+#include <cuda_runtime.h>
+
+namespace krt {
+
+// One layer-major cache: [n_layers][2][n_pages][n_kv_heads][page_size][head],
+// K at 0 and V at 1 of the second axis, bf16 or f32.
+struct PagesView {
+    void *kv;
+    int f32;
+    int n_layers, n_pages, kv_heads, heads, group, head, page_shift;
+    const int32_t *table;  // [max_seqs][max_pages] page ids
+    int max_pages;
+};
+
+// One sequence of the current step: its `rows` new positions ctx .. ctx +
+// rows - 1 are rows row0 .. of the step's q, k, v and out.
+struct StepSeq {
+    int32_t slot, ctx, rows, row0;
+    // table entries [dirty, dirty + n_dirty) come from delta[delta ..]
+    int32_t dirty, n_dirty, delta, pad;
+};
+
+// Page copies (PageCopy of pages.h): src, dst, rows.
+struct CopyItem {
+    int32_t src, dst, rows;
+};
+
+// staged: StepSeq[n], then the table deltas; copies the descriptors to `seqs`
+// and the deltas into the table.
+cudaError_t launch_pages_step(const StepSeq *staged, int n, StepSeq *seqs, int32_t *table, int max_pages,
+                              cudaStream_t s);
+// Row r of k and v [rows, kv_heads * head] f32 into its position of `layer`.
+cudaError_t launch_pages_write(const PagesView &p, int layer, const StepSeq *seqs, int n, int rows, const float *k,
+                               const float *v, cudaStream_t s);
+cudaError_t launch_pages_copy(const PagesView &p, const CopyItem *items, int n, cudaStream_t s);
+// out[r, h] = softmax(q[r, h] . K / sqrt(head)) V over positions 0 .. ctx + i
+// of the row's sequence.
+cudaError_t launch_pages_attention_rows(const PagesView &p, int layer, const StepSeq *seqs, int n, int rows,
+                                        const float *q, float *out, cudaStream_t s);
+
+// Per row of x [rows, vocab]: the target's log probability, the entropy, and
+// the `top` largest (ids ascending among equals) with their log probabilities.
+cudaError_t launch_logprobs(const float *x, int rows, int vocab, const int32_t *targets, float *logprob,
+                            float *entropy, int top, int32_t *top_ids, float *top_logprobs, int *err, cudaStream_t s);
+
+}  // namespace krt

@@ -29,3 +29,17 @@ def as_torch(backend, buf: int, shape, dtype=np.float32, device: int = 0):
     import torch
 
     return torch.as_tensor(_CudaArray(backend.device_ptr(buf), shape, dtype), device=f"cuda:{device}")
+
+
+def pages_as_torch(backend, pages: int, device: int = 0):
+    """A torch tensor aliasing a paged cache, [n_layers, 2, n_pages, n_kv_heads,
+    page_size, head_size], f32 or bf16."""
+    import torch
+
+    from kernrt_b200 import F32
+
+    i = backend.pages_ptr(pages)
+    shape = (i.n_layers, 2, i.n_pages, i.n_kv_heads, i.page_size, i.head_size)
+    dtype = np.float32 if i.kind == F32 else np.uint16
+    t = torch.as_tensor(_CudaArray(i.kv, shape, dtype), device=f"cuda:{device}")
+    return t if i.kind == F32 else t.view(torch.bfloat16)

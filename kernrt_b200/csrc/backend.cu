@@ -1352,12 +1352,21 @@ public:
         StepSeq *seqs = nullptr;  // the current step's descriptors [max_seqs]
         bool stepped = false;     // a step is planned and its tables are current
         size_t n = 0, rows = 0;   // its sequences (those with rows) and rows
+        // the attention's pieces of the step and their scratch, grown as needed
+        AttnItem *items = nullptr;
+        size_t items_cap = 0, n_decode = 0;
+        AttnScratch scratch{};
+        size_t scratch_cap = 0, joins_cap = 0;  // in pieces and in joins
     };
 
     static void free_cache(PagedCache &c) {
         cudaFree(c.view.kv);
         cudaFree(c.table);
         cudaFree(c.seqs);
+        cudaFree(c.items);
+        cudaFree(c.scratch.o);
+        cudaFree(c.scratch.ml);
+        cudaFree(c.scratch.count);
         c = PagedCache{};
     }
 
@@ -1477,6 +1486,65 @@ public:
         return moves.size();
     }
 
+    // The attention's pieces: rows in groups, lengths cut so that the pieces
+    // fill the SMs and no warp sums more than a few hundred keys in a row.
+    static std::vector<AttnItem> plan_attention(const PagesView &v, const std::vector<StepSeq> &desc, size_t *parts,
+                                                size_t *joins) {
+        const size_t slots = (size_t)device_sms() * 4 / (size_t)v.kv_heads;
+        size_t total = 0;
+        for (const StepSeq &d : desc) {
+            const size_t groups = ((size_t)d.rows * v.group + kDecodeRows - 1) / kDecodeRows;
+            total += groups * (size_t)(d.ctx + d.rows);
+        }
+        const size_t share = std::min<size_t>(1024, total / std::max<size_t>(slots, 1) + 1);
+        const int cut = (int)((share + kDecodeKeys - 1) / kDecodeKeys * kDecodeKeys);
+        std::vector<AttnItem> items;
+        for (size_t i = 0; i < desc.size(); ++i) {
+            const StepSeq &d = desc[i];
+            const int m = d.rows * v.group;
+            for (int row = 0; row < m; row += kDecodeRows) {
+                const int rows = std::min(kDecodeRows, m - row);
+                const int hi = d.ctx + (row + rows - 1) / v.group + 1;
+                const int n = (hi + cut - 1) / cut;
+                const int first = (int)items.size(), join = n > 1 ? (int)(*joins)++ : 0;
+                for (int k = 0; k < n; ++k)
+                    items.push_back({(int32_t)i, row, rows, k * cut, std::min(hi, (k + 1) * cut), first, n, join});
+                if (n > 1) *parts = items.size();
+            }
+        }
+        return items;
+    }
+
+    // Room for the step's pieces (memory grown under queued work is freed
+    // after it; counters start, and stay between launches, at 0).
+    void grow_plan(PagedCache &c, size_t items, size_t parts, size_t joins) {
+        const size_t hk = (size_t)c.view.kv_heads;
+        const auto regrow = [&](auto *&ptr, size_t bytes, const char *what) {
+            cudaFree(ptr);
+            ptr = nullptr;
+            check(cudaMalloc(&ptr, bytes), what);
+        };
+        if (items > c.items_cap) {
+            const size_t cap = std::max<size_t>(64, 2 * items);
+            c.items_cap = 0;
+            regrow(c.items, cap * sizeof(AttnItem), "cudaMalloc(attention items)");
+            c.items_cap = cap;
+        }
+        if (parts > c.scratch_cap) {
+            const size_t rows = parts * hk * kDecodeRows;
+            c.scratch_cap = 0;
+            regrow(c.scratch.o, rows * c.view.head * sizeof(float), "cudaMalloc(attention scratch)");
+            regrow(c.scratch.ml, rows * sizeof(float2), "cudaMalloc(attention scratch)");
+            c.scratch_cap = parts;
+        }
+        if (joins > c.joins_cap) {
+            c.joins_cap = 0;
+            regrow(c.scratch.count, joins * hk * sizeof(unsigned), "cudaMalloc(attention scratch)");
+            check(cudaMemsetAsync(c.scratch.count, 0, joins * hk * sizeof(unsigned), stream_), "cudaMemset");
+            c.joins_cap = joins;
+        }
+    }
+
     // The next step of the sequences: each grows by its rows, its table goes
     // up to date on the device, and the step's descriptors are laid down for
     // every layer's pages_write and pages_attention.
@@ -1517,12 +1585,19 @@ public:
         c.n = desc.size();
         c.rows = row0;
         if (c.n) {
-            std::vector<char> block(desc.size() * sizeof(StepSeq) + delta.size() * sizeof(int32_t));
-            std::memcpy(block.data(), desc.data(), desc.size() * sizeof(StepSeq));
-            if (!delta.empty())
-                std::memcpy(block.data() + desc.size() * sizeof(StepSeq), delta.data(), delta.size() * sizeof(int32_t));
+            size_t parts = 0, joins = 0;
+            const std::vector<AttnItem> items = plan_attention(c.view, desc, &parts, &joins);
+            c.n_decode = items.size();
+            grow_plan(c, items.size(), parts, joins);
+            const size_t a = desc.size() * sizeof(StepSeq), b = items.size() * sizeof(AttnItem);
+            std::vector<char> block(a + b + delta.size() * sizeof(int32_t));
+            std::memcpy(block.data(), desc.data(), a);
+            std::memcpy(block.data() + a, items.data(), b);
+            if (!delta.empty()) std::memcpy(block.data() + a + b, delta.data(), delta.size() * sizeof(int32_t));
             const auto *d = static_cast<const StepSeq *>(stage(block.data(), block.size()));
-            launch_or_fail(launch_pages_step(d, (int)c.n, c.seqs, c.table, c.view.max_pages, stream_), "pages_step");
+            launch_or_fail(launch_pages_step(d, (int)c.n, (int)items.size(), c.seqs, c.items, c.table,
+                                             c.view.max_pages, stream_),
+                           "pages_step");
             for (const StepSeq &d2 : desc) c.map->at((size_t)d2.slot).dirty = c.map->at((size_t)d2.slot).pages.size();
         }
         c.stepped = true;
@@ -1554,8 +1629,9 @@ public:
         span(qb, 0, c.rows * width, "pages_attention q");
         span(ob, 0, c.rows * width, "pages_attention out");
         flush();
-        launch_or_fail(launch_pages_attention_rows(c.view, (int)layer, c.seqs, (int)c.n, (int)c.rows, f(qb), f(ob),
-                                                   stream_),
+        if (c.rows == 0) return;
+        launch_or_fail(launch_pages_decode(c.view, (int)layer, c.seqs, c.items, (int)c.n_decode, c.scratch, f(qb),
+                                           f(ob), stream_),
                        "pages_attention");
     }
 

@@ -27,23 +27,43 @@ struct StepSeq {
     int32_t dirty, n_dirty, delta, pad;
 };
 
+// A piece of the step's attention for one kv head: `rows` query rows from `row`
+// on (row = token * group + head of the group) of sequence `seq` of the step
+// over its positions [lo, hi).  n_parts pieces with the same rows, first ..
+// first + n_parts - 1, share the sequence's length and are joined; `join` is
+// the place of their counter.
+struct AttnItem {
+    int32_t seq, row, rows, lo, hi, first, n_parts, join;
+};
+
+// Partial results of the pieces: per (piece, kv head, row of the piece) the
+// values o [head] and (m, l), and per (join, kv head) a counter that is 0
+// between launches.
+struct AttnScratch {
+    float *o;
+    float2 *ml;
+    unsigned *count;
+};
+
 // Page copies (PageCopy of pages.h): src, dst, rows.
 struct CopyItem {
     int32_t src, dst, rows;
 };
 
-// staged: StepSeq[n], then the table deltas; copies the descriptors to `seqs`
-// and the deltas into the table.
-cudaError_t launch_pages_step(const StepSeq *staged, int n, StepSeq *seqs, int32_t *table, int max_pages,
-                              cudaStream_t s);
+// staged: StepSeq[n], AttnItem[n_items], then the table deltas; copies the
+// descriptors to `seqs`, the items to `items` and the deltas into the table.
+cudaError_t launch_pages_step(const StepSeq *staged, int n, int n_items, StepSeq *seqs, AttnItem *items,
+                              int32_t *table, int max_pages, cudaStream_t s);
 // Row r of k and v [rows, kv_heads * head] f32 into its position of `layer`.
 cudaError_t launch_pages_write(const PagesView &p, int layer, const StepSeq *seqs, int n, int rows, const float *k,
                                const float *v, cudaStream_t s);
 cudaError_t launch_pages_copy(const PagesView &p, const CopyItem *items, int n, cudaStream_t s);
 // out[r, h] = softmax(q[r, h] . K / sqrt(head)) V over positions 0 .. ctx + i
-// of the row's sequence.
-cudaError_t launch_pages_attention_rows(const PagesView &p, int layer, const StepSeq *seqs, int n, int rows,
-                                        const float *q, float *out, cudaStream_t s);
+// of the row's sequence, for pieces of at most kDecodeRows rows.
+constexpr int kDecodeRows = 8;
+constexpr int kDecodeKeys = 64;  // positions a CTA takes at once: what splits are rounded to
+cudaError_t launch_pages_decode(const PagesView &p, int layer, const StepSeq *seqs, const AttnItem *items, int n_items,
+                                const AttnScratch &scratch, const float *q, float *out, cudaStream_t s);
 
 // Per row of x [rows, vocab]: the target's log probability, the entropy, and
 // the `top` largest (ids ascending among equals) with their log probabilities.

@@ -42,7 +42,7 @@ struct RowAcc {
     float m, l;
     float o[kHeadMax / 32];
 };
-__device__ inline RowAcc attend_row(const PagesView &p, int layer, int j, const int32_t *table, const float *q, int lo,
+static __device__ __noinline__ RowAcc attend_row(const PagesView &p, int layer, int j, const int32_t *table, const float *q, int lo,
                                     int hi) {
     const int lane = threadIdx.x & 31;
     const int mask = (1 << p.page_shift) - 1;

@@ -1353,10 +1353,12 @@ public:
         bool stepped = false;     // a step is planned and its tables are current
         size_t n = 0, rows = 0;   // its sequences (those with rows) and rows
         // the attention's pieces of the step and their scratch, grown as needed
+        // (decode: pieces of few rows, prompt: of many)
         AttnItem *items = nullptr;
-        size_t items_cap = 0, n_decode = 0;
-        AttnScratch scratch{};
-        size_t scratch_cap = 0, joins_cap = 0;  // in pieces and in joins
+        size_t items_cap = 0, n_decode = 0, n_prompt = 0;
+        bool split_prompt = false;
+        AttnScratch decode{}, prompt{};
+        size_t decode_cap = 0, joins_cap = 0, prompt_cap = 0;  // in pieces, joins, pieces
     };
 
     static void free_cache(PagedCache &c) {
@@ -1364,9 +1366,11 @@ public:
         cudaFree(c.table);
         cudaFree(c.seqs);
         cudaFree(c.items);
-        cudaFree(c.scratch.o);
-        cudaFree(c.scratch.ml);
-        cudaFree(c.scratch.count);
+        for (AttnScratch *w : {&c.decode, &c.prompt}) {
+            cudaFree(w->o);
+            cudaFree(w->ml);
+            cudaFree(w->count);
+        }
         c = PagedCache{};
     }
 
@@ -1486,43 +1490,109 @@ public:
         return moves.size();
     }
 
-    // The attention's pieces: rows in groups, lengths cut so that the pieces
-    // fill the SMs and no warp sums more than a few hundred keys in a row.
-    static std::vector<AttnItem> plan_attention(const PagesView &v, const std::vector<StepSeq> &desc, size_t *parts,
-                                                size_t *joins) {
-        const size_t slots = (size_t)device_sms() * 4 / (size_t)v.kv_heads;
-        size_t total = 0;
-        for (const StepSeq &d : desc) {
-            const size_t groups = ((size_t)d.rows * v.group + kDecodeRows - 1) / kDecodeRows;
-            total += groups * (size_t)(d.ctx + d.rows);
-        }
-        const size_t share = std::min<size_t>(1024, total / std::max<size_t>(slots, 1) + 1);
+    // The step's attention cut into pieces.  A sequence with at most
+    // kFewRows query rows per kv head goes to the kernel for single tokens (groups
+    // of 8 rows that each read the keys again), one with more to the tensor
+    // cores' (256 rows; a piece costs 128 or more whatever it holds).
+    struct AttnPlan {
+        std::vector<AttnItem> decode, prompt;
+        size_t decode_parts = 0, joins = 0, prompt_parts = 0;
+    };
+    static constexpr int kFewRows = 16;
+
+    static AttnPlan plan_attention(const PagesView &v, const std::vector<StepSeq> &desc) {
+        AttnPlan a;
+        const size_t sms = (size_t)device_sms(), hk = (size_t)v.kv_heads;
+        size_t keys = 0;
+        for (const StepSeq &d : desc)
+            if (d.rows * v.group <= kFewRows)
+                keys += (size_t)((d.rows * v.group + kDecodeRows - 1) / kDecodeRows) * (size_t)(d.ctx + d.rows);
+        // pieces of about as many keys as fill every SM four times, and of at
+        // most 1024, so that a warp sums no more than 256 keys in a row
+        const size_t share = std::min<size_t>(1024, keys * hk / (4 * sms) + 1);
         const int cut = (int)((share + kDecodeKeys - 1) / kDecodeKeys * kDecodeKeys);
-        std::vector<AttnItem> items;
         for (size_t i = 0; i < desc.size(); ++i) {
             const StepSeq &d = desc[i];
             const int m = d.rows * v.group;
-            for (int row = 0; row < m; row += kDecodeRows) {
-                const int rows = std::min(kDecodeRows, m - row);
+            const int step = m <= kFewRows ? kDecodeRows : kPromptRows;
+            for (int row = 0; row < m; row += step) {
+                const int rows = std::min(step, m - row);
                 const int hi = d.ctx + (row + rows - 1) / v.group + 1;
+                if (m > kFewRows) {
+                    a.prompt.push_back({(int32_t)i, row, rows, 0, hi, 0, 1, 0});
+                    continue;
+                }
                 const int n = (hi + cut - 1) / cut;
-                const int first = (int)items.size(), join = n > 1 ? (int)(*joins)++ : 0;
+                const int first = (int)a.decode.size(), join = n > 1 ? (int)a.joins++ : 0;
                 for (int k = 0; k < n; ++k)
-                    items.push_back({(int32_t)i, row, rows, k * cut, std::min(hi, (k + 1) * cut), first, n, join});
-                if (n > 1) *parts = items.size();
+                    a.decode.push_back({(int32_t)i, row, rows, k * cut, std::min(hi, (k + 1) * cut), first, n, join});
+                if (n > 1) a.decode_parts = a.decode.size();
             }
         }
-        return items;
+        // the longest pieces first
+        std::stable_sort(a.prompt.begin(), a.prompt.end(),
+                         [](const AttnItem &x, const AttnItem &y) { return x.hi > y.hi; });
+        for (size_t i = 0; i < a.prompt.size(); ++i) a.prompt[i].first = (int32_t)i;
+        split_prompts(a, sms, hk);
+        return a;
+    }
+
+    // Few and long pieces (a chunk behind a long context) are cut so that they
+    // fill the SMs: of the piece lengths from the longest down, the one whose
+    // pieces, dealt out longest first, end soonest.  A piece costs its key
+    // tiles and about three more for its query rows, its start and its join.
+    static void split_prompts(AttnPlan &a, size_t sms, size_t hk) {
+        if (a.prompt.empty() || a.prompt.size() * hk >= 2 * sms) return;
+        constexpr int kPieceCost = 3;
+        const auto tiles = [](const AttnItem &x) { return (x.hi + kPromptKeys - 1) / kPromptKeys; };
+        const int longest = tiles(a.prompt[0]);
+        int best_cut = longest;
+        long best = -1;
+        for (int parts = 1, last = 0; parts <= 64 && parts <= longest; ++parts) {
+            const int cut = (longest + parts - 1) / parts;
+            if (cut == last || cut < 4) continue;
+            last = cut;
+            size_t pieces = 0;
+            long sum = 0, most = 0;
+            for (const AttnItem &x : a.prompt) {
+                const int n = (tiles(x) + cut - 1) / cut, each = (tiles(x) + n - 1) / n;
+                pieces += (size_t)n;
+                sum += tiles(x) + n * kPieceCost;
+                most = std::max<long>(most, each + kPieceCost);
+            }
+            const long rounds = (long)((pieces * hk + sms - 1) / sms);
+            // between even shares and whole rounds of the longest
+            const long cost = std::max(most, std::min(rounds * most, (long)((size_t)sum * hk / sms) + most));
+            if (best < 0 || cost < best) best = cost, best_cut = cut;
+        }
+        if (best_cut >= longest) return;
+        std::vector<AttnItem> cut;
+        for (const AttnItem &x : a.prompt) {
+            const int n = (tiles(x) + best_cut - 1) / best_cut, each = (tiles(x) + n - 1) / n;
+            const int first = (int)cut.size(), parts = (tiles(x) + each - 1) / each;
+            for (int k = 0; k < parts; ++k)
+                cut.push_back({x.seq, x.row, x.rows, k * each * kPromptKeys, std::min(x.hi, (k + 1) * each * kPromptKeys),
+                               first, parts, 0});
+            if (parts > 1) a.prompt_parts = cut.size();
+        }
+        a.prompt = std::move(cut);
     }
 
     // Room for the step's pieces (memory grown under queued work is freed
     // after it; counters start, and stay between launches, at 0).
-    void grow_plan(PagedCache &c, size_t items, size_t parts, size_t joins) {
-        const size_t hk = (size_t)c.view.kv_heads;
+    void grow_plan(PagedCache &c, const AttnPlan &a) {
+        const size_t hk = (size_t)c.view.kv_heads, items = a.decode.size() + a.prompt.size();
         const auto regrow = [&](auto *&ptr, size_t bytes, const char *what) {
             cudaFree(ptr);
             ptr = nullptr;
             check(cudaMalloc(&ptr, bytes), what);
+        };
+        const auto scratch = [&](AttnScratch &w, size_t &cap, size_t parts, size_t rows) {
+            if (parts <= cap) return;
+            cap = 0;
+            regrow(w.o, parts * hk * rows * c.view.head * sizeof(float), "cudaMalloc(attention scratch)");
+            regrow(w.ml, parts * hk * rows * sizeof(float2), "cudaMalloc(attention scratch)");
+            cap = parts;
         };
         if (items > c.items_cap) {
             const size_t cap = std::max<size_t>(64, 2 * items);
@@ -1530,18 +1600,13 @@ public:
             regrow(c.items, cap * sizeof(AttnItem), "cudaMalloc(attention items)");
             c.items_cap = cap;
         }
-        if (parts > c.scratch_cap) {
-            const size_t rows = parts * hk * kDecodeRows;
-            c.scratch_cap = 0;
-            regrow(c.scratch.o, rows * c.view.head * sizeof(float), "cudaMalloc(attention scratch)");
-            regrow(c.scratch.ml, rows * sizeof(float2), "cudaMalloc(attention scratch)");
-            c.scratch_cap = parts;
-        }
-        if (joins > c.joins_cap) {
+        scratch(c.decode, c.decode_cap, a.decode_parts, kDecodeRows);
+        scratch(c.prompt, c.prompt_cap, a.prompt_parts, kPromptRows);
+        if (a.joins > c.joins_cap) {
             c.joins_cap = 0;
-            regrow(c.scratch.count, joins * hk * sizeof(unsigned), "cudaMalloc(attention scratch)");
-            check(cudaMemsetAsync(c.scratch.count, 0, joins * hk * sizeof(unsigned), stream_), "cudaMemset");
-            c.joins_cap = joins;
+            regrow(c.decode.count, a.joins * hk * sizeof(unsigned), "cudaMalloc(attention scratch)");
+            check(cudaMemsetAsync(c.decode.count, 0, a.joins * hk * sizeof(unsigned), stream_), "cudaMemset");
+            c.joins_cap = a.joins;
         }
     }
 
@@ -1585,18 +1650,26 @@ public:
         c.n = desc.size();
         c.rows = row0;
         if (c.n) {
-            size_t parts = 0, joins = 0;
-            const std::vector<AttnItem> items = plan_attention(c.view, desc, &parts, &joins);
-            c.n_decode = items.size();
-            grow_plan(c, items.size(), parts, joins);
-            const size_t a = desc.size() * sizeof(StepSeq), b = items.size() * sizeof(AttnItem);
-            std::vector<char> block(a + b + delta.size() * sizeof(int32_t));
-            std::memcpy(block.data(), desc.data(), a);
-            std::memcpy(block.data() + a, items.data(), b);
-            if (!delta.empty()) std::memcpy(block.data() + a + b, delta.data(), delta.size() * sizeof(int32_t));
+            const AttnPlan plan = plan_attention(c.view, desc);
+            grow_plan(c, plan);
+            c.n_decode = plan.decode.size();
+            c.n_prompt = plan.prompt.size();
+            c.split_prompt = plan.prompt_parts > 0;
+            const size_t n_items = c.n_decode + c.n_prompt;
+            std::vector<char> block(desc.size() * sizeof(StepSeq) + n_items * sizeof(AttnItem) +
+                                    delta.size() * sizeof(int32_t));
+            char *to = block.data();
+            const auto put = [&](const void *src, size_t bytes) {
+                if (bytes) std::memcpy(to, src, bytes);
+                to += bytes;
+            };
+            put(desc.data(), desc.size() * sizeof(StepSeq));
+            put(plan.decode.data(), c.n_decode * sizeof(AttnItem));
+            put(plan.prompt.data(), c.n_prompt * sizeof(AttnItem));
+            put(delta.data(), delta.size() * sizeof(int32_t));
             const auto *d = static_cast<const StepSeq *>(stage(block.data(), block.size()));
-            launch_or_fail(launch_pages_step(d, (int)c.n, (int)items.size(), c.seqs, c.items, c.table,
-                                             c.view.max_pages, stream_),
+            launch_or_fail(launch_pages_step(d, (int)c.n, (int)n_items, c.seqs, c.items, c.table, c.view.max_pages,
+                                             stream_),
                            "pages_step");
             for (const StepSeq &d2 : desc) c.map->at((size_t)d2.slot).dirty = c.map->at((size_t)d2.slot).pages.size();
         }
@@ -1630,9 +1703,12 @@ public:
         span(ob, 0, c.rows * width, "pages_attention out");
         flush();
         if (c.rows == 0) return;
-        launch_or_fail(launch_pages_decode(c.view, (int)layer, c.seqs, c.items, (int)c.n_decode, c.scratch, f(qb),
+        launch_or_fail(launch_pages_decode(c.view, (int)layer, c.seqs, c.items, (int)c.n_decode, c.decode, f(qb),
                                            f(ob), stream_),
                        "pages_attention");
+        launch_or_fail(launch_pages_prompt(c.view, (int)layer, c.seqs, c.items + c.n_decode, (int)c.n_prompt,
+                                           c.split_prompt, c.prompt, f(qb), f(ob), d_err_, stream_),
+                       "pages_attention (tensor cores)");
     }
 
     // ---- log probabilities of given tokens (logprobs.cu) ------------------------

@@ -65,6 +65,14 @@ constexpr int kDecodeKeys = 64;  // positions a CTA takes at once: what splits a
 cudaError_t launch_pages_decode(const PagesView &p, int layer, const StepSeq *seqs, const AttnItem *items, int n_items,
                                 const AttnScratch &scratch, const float *q, float *out, cudaStream_t s);
 
+// The same for pieces of many rows (paged_prompt.cu); `split`: some piece has
+// more than one part.
+constexpr int kPromptRows = 256;
+constexpr int kPromptKeys = 128;  // what splits are rounded to
+cudaError_t launch_pages_prompt(const PagesView &p, int layer, const StepSeq *seqs, const AttnItem *items, int n_items,
+                                bool split, const AttnScratch &scratch, const float *q, float *out, int *err,
+                                cudaStream_t s);
+
 // Per row of x [rows, vocab]: the target's log probability, the entropy, and
 // the `top` largest (ids ascending among equals) with their log probabilities.
 cudaError_t launch_logprobs(const float *x, int rows, int vocab, const int32_t *targets, float *logprob,

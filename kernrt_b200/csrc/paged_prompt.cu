@@ -1,0 +1,646 @@
+// Attention of many query rows (whole prompts, chunks) over the paged cache on
+// the tensor cores (tcgen05.mma, accumulators in TMEM).
+//
+// out = softmax(q K^T / sqrt(D)) V per row, one pass over the keys: with m the
+// running maximum of the scores x (in powers of two), weights w = 2^(x - m), l =
+// sum w and acc = sum w V, a larger maximum rescales l and acc by 2^(m_old -
+// m_new), and out = acc / l at the end.  Query rows of one kv head are packed as
+// (token, head of the group), so that a group shares every K and V tile.
+//
+// Precision.  Rows are f32, and one 16-bit operand would round q and the
+// weights to 2^-9 or 2^-11.  Both go in as two fp16 halves (x = hi + lo to
+// 2^-22; fp16 carries three bits more than bf16, so two halves do what takes
+// bf16 three), which doubles the MMA work instead of tripling it.  Both operands
+// of an MMA are then fp16, so the CTA's loader turns page rows into fp16: every
+// tile of K or V is multiplied by the power of two that brings its largest
+// magnitude to [2^13, 2^14), which keeps bf16 values exact down to 2^-28 of the
+// tile's largest, f32 values (as two halves, three products) to 2^-22 of their
+// own and 2^-38 of the tile's largest; query rows likewise, row by row.
+// The scales return as one factor of the scores and one of the tile's sum.
+// Where a tile's magnitudes spread so far that some eight neighbouring elements
+// lie 2^18 below its largest (or it holds an infinity or NaN), the CTA's rows are
+// attended again by attend_row in f32, each over the keys it sees alone; so are
+// rows whose result is not finite.  What stands in masked places (later
+// positions of the same prompt included) therefore never reaches a row.
+// The tensor cores add into an f32 accumulator with truncation: measured
+// relative error 1.1e-9 per K (9e-6 at K = 8192, always toward zero), so
+// a tile's sum of V is taken out of TMEM after every 64 or 128 keys and added in
+// registers with rounding.
+//
+// One CTA: 256 query rows as two M = 128 tiles, so that the softmax of one runs
+// under the MMAs of the other.  Warps 0-3 and 4-7: a thread per row of the two
+// tiles (scores from TMEM, weights back over them in place, acc in registers).
+// Warps 8-11: the loader, global memory to swizzled shared tiles through
+// registers, a ring of tiles K0 V0 K1 V1 ..  Warp 12: one thread issues the MMAs.
+// Every wait is bounded: one that runs out sets ERR_TIMEOUT and the roles stop.
+#include <cuda_fp16.h>
+
+#include "kernels.cuh"
+#include "paged.cuh"
+#include "paged_dev.cuh"
+#include "tcgen.cuh"
+
+namespace krt {
+
+namespace {
+
+constexpr int kRows = kPromptRows;  // query rows of a CTA
+constexpr int kPromptThreads = 512;
+constexpr int kScaleRing = 16;  // tiles' scales; the loader is at most 4 tiles ahead
+
+template <int D, bool F32>
+struct Shape {
+    static constexpr int Keys = F32 && D == 128 ? 64 : 128;  // keys of a tile
+    static constexpr int Parts = F32 ? 2 : 1;                // fp16 halves of K and V
+    static constexpr int Sub = Keys * 128;                   // bytes of a [Keys][64] fp16 sub-tile
+    static constexpr int Slot = Parts * (D / 64) * Sub;
+    static constexpr int Slots = D == 64 ? (F32 ? 4 : 6) : 3;
+    static constexpr int QTile = 2 * (D / 64) * 128 * 128;  // both halves of 128 rows
+    static constexpr size_t Smem = 2 * (size_t)QTile + (size_t)Slots * Slot + 1024;
+    static constexpr int Region = Keys + D;  // TMEM columns of a query tile: scores / weights, sum of V
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Instruction descriptor of kind::f16: D f32 (bits 4-5 = 1), A and B fp16 (bits
+// 7-9, 10-12 = 0), A K-major, B K-major or (bit 16) MN-major, N / 8 at bits
+// 17-22, M / 16 at bits 24-28.
+template <int N, bool MnMajor>
+__host__ __device__ constexpr uint32_t idesc() {
+    return (1u << 4) | (MnMajor ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+// Descriptor of an MN-major tile [K rows][64 of N per sub-tile], 128-byte
+// swizzled: 8-row groups of K 1 KB apart (stride byte offset), 64-wide groups
+// of N `sub` bytes apart (leading byte offset).
+__device__ __forceinline__ uint64_t mn_desc(uint32_t saddr, uint32_t sub) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((sub >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// D += A B with A from shared memory, or from TMEM.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(desc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(desc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ float2 unpack_half(uint32_t v) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+}
+
+// The power of two that brings a magnitude with these bits to [2^13, 2^14), and
+// its inverse (both normal: magnitudes below 2^-112 get 2^126).
+__device__ __forceinline__ float up_scale(uint32_t bits) {
+    const int e = (int)(bits >> 23);
+    return e == 255 ? 1.0f : __uint_as_float((uint32_t)(267 - e < 253 ? 267 - e : 253) << 23);
+}
+__device__ __forceinline__ float down_scale(float up) { return __uint_as_float((254u << 23) - __float_as_uint(up)); }
+
+// Whether magnitudes spread too far for one scale (bits of the largest, and of
+// the smallest non-zero largest-of-eight less 1).
+__device__ __forceinline__ bool too_wide(uint32_t most, uint32_t least_1) {
+    return most >= 0x7f800000u || (most != 0 && (int)(most >> 23) - (int)((least_1 + 1) >> 23) > 18);
+}
+
+// Byte offset of 16-byte chunk c of row r in a 128-byte swizzled sub-tile.
+__device__ __forceinline__ uint32_t swizzled(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
+
+__device__ __forceinline__ void store_shared(uint32_t addr, uint4 v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Eight f32 values times s as fp16: the halves hi and, if wanted, lo.
+template <bool Lo>
+__device__ __forceinline__ void halves(const float (&x)[8], float s, uint4 &hi, uint4 &lo) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float a = x[2 * i] * s, b = x[2 * i + 1] * s;
+        h[i] = pack_half(a, b);
+        if (Lo) {
+            const float2 f = unpack_half(h[i]);
+            l[i] = pack_half(a - f.x, b - f.y);
+        }
+    }
+    hi = make_uint4(h[0], h[1], h[2], h[3]);
+    if (Lo) lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+// Barrier of the loader's 128 threads that also says whether any of them has p.
+__device__ __forceinline__ bool loader_or(bool p) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+        : "=r"(r)
+        : "r"((uint32_t)p)
+        : "memory");
+    return r != 0;
+}
+
+template <int D, bool F32>
+__global__ void __launch_bounds__(kPromptThreads, 1)
+    k_pages_prompt(PagesView p, int layer, const StepSeq *__restrict__ seqs, const AttnItem *__restrict__ items,
+                   AttnScratch scratch, const float *__restrict__ q, float *__restrict__ out, int *err) {
+    using S = Shape<D, F32>;
+    constexpr int Keys = S::Keys;
+    extern __shared__ unsigned char raw_smem[];
+    __shared__ uint64_t slot_full[S::Slots], slot_empty[S::Slots], s_full[2], p_full[2], q_full, done;
+    __shared__ uint32_t s_tmem, s_red[2][4][2];
+    __shared__ float s_kscale[kScaleRing], s_vscale[kScaleRing];
+    __shared__ int s_abort, s_wild;
+    const uint32_t base = (smem_addr(raw_smem) + 1023u) & ~1023u;
+    const uint32_t slots = base + 2 * S::QTile;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile int *abort_flag = &s_abort;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::Slots; ++i) {
+            mbar_init(&slot_full[i], 4);
+            mbar_init(&slot_empty[i], 1);
+        }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&s_full[t], 1);
+            mbar_init(&p_full[t], 4);
+        }
+        mbar_init(&q_full, 8);
+        mbar_init(&done, 1);
+        s_abort = 0;
+        s_wild = 0;
+        mbar_fence_init();
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+
+    const int item = (int)(blockIdx.x / (unsigned)p.kv_heads), j = (int)(blockIdx.x % (unsigned)p.kv_heads);
+    const AttnItem it = items[item];
+    const StepSeq sq = seqs[it.seq];
+    const int32_t *table = p.table + (size_t)sq.slot * p.max_pages;
+    // key tiles of the two query tiles: up to the last position any row sees
+    int n_tiles[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int last = min(it.rows, 128 * (t + 1)) - 1;
+        const int seen = min(it.hi, sq.ctx + (it.row + last) / p.group + 1) - it.lo;
+        n_tiles[t] = last < 128 * t || seen <= 0 ? 0 : (seen + Keys - 1) / Keys;
+    }
+    const int n = max(n_tiles[0], n_tiles[1]);
+
+    const auto wait = [&](uint64_t *bar, int phase) {
+        if (mbar_try_wait(bar, (uint32_t)phase & 1u)) return true;
+        const long long t0 = clock64();
+        while (!mbar_try_wait(bar, (uint32_t)phase & 1u)) {
+            if (*abort_flag) return false;
+            if (clock64() - t0 > (1ll << 31)) {
+                if (err) atomicOr(err, ERR_TIMEOUT);
+                *abort_flag = 1;
+                return false;
+            }
+        }
+        return true;
+    };
+
+    if (warp < 8) {
+        // ---- a thread per query row -----------------------------------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        const int t = warp >> 2, r = threadIdx.x;  // r = 128 t + row of the tile
+        const bool live = r < it.rows;
+        const int m_row = it.row + (live ? r : 0), token = m_row / p.group;
+        const size_t at =
+            ((size_t)(sq.row0 + token) * p.heads + (size_t)j * p.group + (m_row - token * p.group)) * p.head;
+        const int limit = live ? min(it.hi, sq.ctx + token + 1) : it.lo;
+        float sc;
+        {  // the row's halves, scaled to its largest element
+            const int chunks = p.head >> 3;
+            const float4 *src = reinterpret_cast<const float4 *>(q + at);
+            uint32_t most = 0, least = 0xffffffffu;
+#pragma unroll 4
+            for (int c = 0; c < D / 8; ++c) {
+                if (!live || c >= chunks) break;
+                const float4 a = __ldg(src + 2 * c), b = __ldg(src + 2 * c + 1);
+                const float x = fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w)));
+                const float y = fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w)));
+                uint32_t m = __float_as_uint(fmaxf(x, y));
+                const float z = ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
+                if (z != z) m = 0x7f800000u;  // NaN, or infinities of both signs
+                most = max(most, m);
+                least = min(least, m - 1);
+            }
+            if (too_wide(most, least)) s_wild = 1;
+            const float up = up_scale(most);
+            sc = kLog2e * rsqrtf((float)p.head) * down_scale(up);
+            const uint32_t tile = base + (uint32_t)t * S::QTile;
+#pragma unroll 2
+            for (int c = 0; c < D / 8; ++c) {
+                float x[8] = {};
+                if (live && c < chunks) {
+                    const float4 a = __ldg(src + 2 * c), b = __ldg(src + 2 * c + 1);
+                    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+                    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+                }
+                uint4 hi, lo;
+                halves<true>(x, up, hi, lo);
+                const uint32_t o = tile + (uint32_t)(c >> 3) * 16384 + swizzled(r & 127, c & 7);
+                store_shared(o, hi);
+                store_shared(o + (D / 64) * 16384, lo);
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full);
+        }
+
+        float acc[D];
+#pragma unroll
+        for (int d = 0; d < D; ++d) acc[d] = 0.0f;
+        float m = -INFINITY, l = 0.0f;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t s_at = tmem + lanes + (uint32_t)(t * S::Region), o_at = s_at + Keys;
+        const auto flush = [&](int tile) {  // the tile's sum of V into the registers
+            const float vs = s_vscale[tile & (kScaleRing - 1)];
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+                uint32_t v[32];
+                tmem_ld32(o_at + (uint32_t)c, v);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) acc[c + i] = __fmaf_rn(__uint_as_float(v[i]), vs, acc[c + i]);
+            }
+        };
+        bool ok = true;
+        const int mine = n_tiles[t];
+        for (int tile = 0; tile < mine; ++tile) {
+            ok = __all_sync(0xffffffffu, wait(&s_full[t], tile));
+            if (!ok) break;
+            tc_fence_after();
+            const int rem = limit - (it.lo + tile * Keys);  // the tile's keys this row sees
+            const bool masked = __any_sync(0xffffffffu, rem < Keys);
+            const float ks = sc * s_kscale[tile & (kScaleRing - 1)];
+            float mx = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < Keys; c += 32) {
+                uint32_t v[32];
+                tmem_ld32(s_at + (uint32_t)c, v);
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (c + i < rem) mx = fmaxf(mx, __uint_as_float(v[i]));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(v[i]));
+                }
+            }
+            if (tile) flush(tile - 1);
+            const float mn = fmaxf(m, mx * ks);
+            if (tile && __any_sync(0xffffffffu, mn > m)) {
+                const float keep = mn == -INFINITY ? 0.0f : ex2(m - mn);
+                l *= keep;
+#pragma unroll
+                for (int d = 0; d < D; ++d) acc[d] *= keep;
+            }
+            m = mn;
+            // weights times 2^14: the halves of small ones stay normal numbers
+            const float bias = 14.0f - (m == -INFINITY ? 0.0f : m);
+            float sum = 0.0f;
+#pragma unroll
+            for (int c = 0; c < Keys; c += 32) {
+                uint32_t v[32];
+                tmem_ld32(s_at + (uint32_t)c, v);
+                float w[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) w[i] = ex2(__fmaf_rn(__uint_as_float(v[i]), ks, bias));
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (c + i >= rem) w[i] = 0.0f;
+                }
+                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < 32; ++i) part[i & 3] += w[i];
+                sum += (part[0] + part[1]) + (part[2] + part[3]);
+                // in place: 16 columns of the halves hi, 16 of lo
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    v[i] = pack_half(w[2 * i], w[2 * i + 1]);
+                    const float2 f = unpack_half(v[i]);
+                    v[16 + i] = pack_half(w[2 * i] - f.x, w[2 * i + 1] - f.y);
+                }
+                tmem_st32(s_at + (uint32_t)c, v);
+            }
+            l += sum;
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[t]);
+        }
+        if (ok && mine) {
+            ok = __all_sync(0xffffffffu, wait(&s_full[t], mine));
+            tc_fence_after();
+            if (ok) flush(mine - 1);
+        }
+        if (ok) {
+            bool fine = isfinite(l) && !*(volatile int *)&s_wild;
+#pragma unroll
+            for (int d = 0; d < D; ++d) fine = fine && isfinite(acc[d]);
+            const size_t part = ((size_t)item * p.kv_heads + j) * kRows + r;
+            if (live && fine) {
+                const float f = it.n_parts == 1 ? 1.0f / l : 0x1p-14f;
+                float4 *dst = reinterpret_cast<float4 *>(it.n_parts == 1 ? out + at : scratch.o + part * p.head);
+#pragma unroll
+                for (int d = 0; d < D; d += 4)
+                    if (d < p.head) dst[d / 4] = make_float4(acc[d] * f, acc[d + 1] * f, acc[d + 2] * f, acc[d + 3] * f);
+                if (it.n_parts > 1) scratch.ml[part] = make_float2(m, l * 0x1p-14f);
+            }
+            unsigned again = __ballot_sync(0xffffffffu, live && !fine);
+            while (again) {
+                const int w = __ffs((int)again) - 1;
+                again &= again - 1;
+                const size_t at_w = __shfl_sync(0xffffffffu, at, w), part_w = __shfl_sync(0xffffffffu, part, w);
+                const RowAcc a = attend_row(p, layer, j, table, q + at_w, it.lo, __shfl_sync(0xffffffffu, limit, w));
+#pragma unroll
+                for (int i = 0; i < kHeadMax / 32; ++i) {
+                    const int d = lane + 32 * i;
+                    if (d >= p.head) continue;
+                    if (it.n_parts == 1) out[at_w + d] = a.o[i] / a.l;
+                    else scratch.o[part_w * p.head + d] = a.o[i];
+                }
+                if (it.n_parts > 1 && lane == 0) scratch.ml[part_w] = make_float2(a.m, a.l);
+            }
+        }
+    } else if (warp < 12) {
+        // ---- the loader: tiles K0 V0 K1 V1 .. ---------------------------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        constexpr int PerRow = D / 8, Step = 128 / PerRow;  // eight-element chunks of a row, rows of a step
+        constexpr int Loads = Keys / Step;
+        const int tid = threadIdx.x - 256, chunk = tid % PerRow, row = tid / PerRow;
+        const bool have = chunk < (p.head >> 3);
+        const int page_mask = (1 << p.page_shift) - 1;
+        const size_t page_stride = (size_t)p.kv_heads * ((size_t)p.head << p.page_shift);
+        const size_t v_off = page_elem(p, layer, 1, 0, j) - page_elem(p, layer, 0, 0, j);
+        const size_t k_base = page_elem(p, layer, 0, 0, j) + 8 * chunk;
+        int pages = 0;  // lane i: the page of positions 16 i .. of the tile
+        for (int i = 0; i < 2 * n; ++i) {
+            const int key0 = it.lo + (i >> 1) * Keys, slot = i % S::Slots;
+            if (!(i & 1)) {
+                const int pos = key0 + 16 * lane;
+                pages = lane < Keys / 16 && pos < it.hi ? __ldg(table + (pos >> p.page_shift)) : 0;
+            }
+            const size_t tile_base = k_base + ((i & 1) ? v_off : 0);
+            uint4 v[Loads * (F32 ? 2 : 1)];
+#pragma unroll
+            for (int k = 0; k < Loads; ++k) {
+                const int pos = key0 + k * Step + row;
+                const int page = __shfl_sync(0xffffffffu, pages, k * Step / 16);
+                const size_t e = tile_base + (size_t)page * page_stride + (size_t)(pos & page_mask) * p.head;
+                const bool in = have && pos < it.hi;
+                const uint4 zero = make_uint4(0, 0, 0, 0);
+                if constexpr (F32) {
+                    const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const float *>(p.kv) + e);
+                    v[2 * k] = in ? __ldg(src) : zero;
+                    v[2 * k + 1] = in ? __ldg(src + 1) : zero;
+                } else {
+                    v[k] = in ? __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.kv) + e)) : zero;
+                }
+            }
+            // the tile's largest magnitude, and the smallest of the chunks'
+            uint32_t most = 0, least = 0xffffffffu;
+#pragma unroll
+            for (int k = 0; k < Loads; ++k) {
+                uint32_t m;
+                if constexpr (F32) {
+                    const uint32_t a = max(max(v[2 * k].x & 0x7fffffffu, v[2 * k].y & 0x7fffffffu),
+                                           max(v[2 * k].z & 0x7fffffffu, v[2 * k].w & 0x7fffffffu));
+                    const uint32_t b = max(max(v[2 * k + 1].x & 0x7fffffffu, v[2 * k + 1].y & 0x7fffffffu),
+                                           max(v[2 * k + 1].z & 0x7fffffffu, v[2 * k + 1].w & 0x7fffffffu));
+                    m = max(a, b);
+                } else {
+                    const uint32_t a = __vmaxu2(v[k].x & 0x7fff7fffu, v[k].y & 0x7fff7fffu);
+                    const uint32_t b = __vmaxu2(v[k].z & 0x7fff7fffu, v[k].w & 0x7fff7fffu);
+                    const uint32_t c = __vmaxu2(a, b);
+                    m = max(c << 16, c & 0xffff0000u);
+                }
+                most = max(most, m);
+                least = min(least, m - 1);
+            }
+            most = __reduce_max_sync(0xffffffffu, most);
+            least = __reduce_min_sync(0xffffffffu, least);
+            uint32_t(&red)[4][2] = s_red[i & 1];
+            if (lane == 0) {
+                red[warp - 8][0] = most;
+                red[warp - 8][1] = least;
+            }
+            const bool ok = i < S::Slots || wait(&slot_empty[slot], i / S::Slots - 1);
+            if (loader_or(!ok)) break;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                most = max(most, red[w][0]);
+                least = min(least, red[w][1]);
+            }
+            const float up = up_scale(most);
+            if (tid == 0) {
+                if (too_wide(most, least)) s_wild = 1;
+                ((i & 1) ? s_vscale : s_kscale)[(i >> 1) & (kScaleRing - 1)] = down_scale(up);
+            }
+            const uint32_t dst = slots + (uint32_t)slot * S::Slot + (uint32_t)(chunk >> 3) * S::Sub;
+#pragma unroll
+            for (int k = 0; k < Loads; ++k) {
+                float x[8];
+                if constexpr (F32) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float((&v[2 * k + (e >> 2)].x)[e & 3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t u = (&v[k].x)[e];
+                        x[2 * e] = __uint_as_float(u << 16);
+                        x[2 * e + 1] = __uint_as_float(u & 0xffff0000u);
+                    }
+                }
+                uint4 hi, lo;
+                halves<F32>(x, up, hi, lo);
+                const uint32_t o = dst + swizzled(k * Step + row, chunk & 7);
+                store_shared(o, hi);
+                if (F32) store_shared(o + (D / 64) * S::Sub, lo);
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&slot_full[slot]);
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
+        if (warp == 12 && lane == 0) {
+            // ---- the MMAs ---------------------------------------------------------
+            const auto scores = [&](int t, int tile) {  // S = (q_hi + q_lo) K^T
+                const uint32_t k = slots + (uint32_t)(2 * tile % S::Slots) * S::Slot, a = base + (uint32_t)t * S::QTile;
+                uint32_t more = 0;
+#pragma unroll 1
+                for (int x = 0; x < S::Parts + 1; ++x) {  // q_hi K_hi, q_lo K_hi, q_hi K_lo
+                    const uint32_t qa = a + (x == 1 ? (D / 64) * 16384 : 0), kb = k + (x == 2 ? (D / 64) * S::Sub : 0);
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d) {
+                        mma_ss(tmem + (uint32_t)(t * S::Region), sw128_desc(qa + (d >> 2) * 16384 + (d & 3) * 32),
+                               sw128_desc(kb + (d >> 2) * S::Sub + (d & 3) * 32), idesc<Keys, false>(), more);
+                        more = 1;
+                    }
+                }
+            };
+            const auto values = [&](int t, int tile) {  // O = (w_hi + w_lo) V
+                const uint32_t v = slots + (uint32_t)((2 * tile + 1) % S::Slots) * S::Slot;
+                const uint32_t w = tmem + (uint32_t)(t * S::Region);
+                uint32_t more = 0;
+#pragma unroll 1
+                for (int x = 0; x < S::Parts + 1; ++x) {  // w_hi V_hi, w_lo V_hi, w_hi V_lo
+                    const uint32_t vb = v + (x == 2 ? (D / 64) * S::Sub : 0);
+#pragma unroll
+                    for (int k = 0; k < Keys / 16; ++k) {
+                        mma_ts(w + Keys, w + (uint32_t)((k >> 1) * 32 + (x == 1 ? 16 : 0) + (k & 1) * 8),
+                               mn_desc(vb + (uint32_t)k * 2048, S::Sub), idesc<D, true>(), more);
+                        more = 1;
+                    }
+                }
+            };
+            const auto full = [&](int i) { return wait(&slot_full[i % S::Slots], i / S::Slots); };
+            bool ok = wait(&q_full, 0) && (n == 0 || full(0));
+            if (ok && n > 0) {
+                tc_fence_after();
+                for (int t = 0; t < 2; ++t)
+                    if (n_tiles[t] > 0) {
+                        scores(t, 0);
+                        mma_commit(&s_full[t]);
+                    }
+                mma_commit(&slot_empty[0]);
+            }
+            for (int tile = 0; ok && tile < n; ++tile) {
+                for (int t = 0; ok && t < 2; ++t) {
+                    if (tile >= n_tiles[t]) continue;
+                    ok = full(2 * tile + 1) && wait(&p_full[t], tile);
+                    if (!ok) break;
+                    tc_fence_after();
+                    values(t, tile);
+                    if (tile + 1 < n_tiles[t]) {
+                        ok = full(2 * tile + 2);
+                        if (!ok) break;
+                        tc_fence_after();
+                        scores(t, tile + 1);
+                    }
+                    mma_commit(&s_full[t]);
+                }
+                if (!ok) break;
+                mma_commit(&slot_empty[(2 * tile + 1) % S::Slots]);
+                if (tile + 1 < n) mma_commit(&slot_empty[(2 * tile + 2) % S::Slots]);
+            }
+            mma_commit(&done);  // every MMA issued, finished loop or not
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        mbar_wait_bounded(&done, 0);  // before the TMEM goes
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// Joins the pieces of split rows, in the order of the pieces: a warp per row.
+__global__ void __launch_bounds__(128) k_pages_join(PagesView p, const StepSeq *__restrict__ seqs,
+                                                    const AttnItem *__restrict__ items, AttnScratch scratch,
+                                                    float *__restrict__ out) {
+    const int item = (int)(blockIdx.x / (unsigned)p.kv_heads), j = (int)(blockIdx.x % (unsigned)p.kv_heads);
+    const AttnItem it = items[item];
+    if (it.n_parts == 1 || it.first != item) return;
+    const StepSeq sq = seqs[it.seq];
+    const int lane = threadIdx.x & 31;
+    for (int r = 4 * blockIdx.y + (threadIdx.x >> 5); r < it.rows; r += 4 * gridDim.y) {
+        const size_t first = ((size_t)it.first * p.kv_heads + j) * kRows + r, step = (size_t)p.kv_heads * kRows;
+        float M = -INFINITY;
+        for (int i = 0; i < it.n_parts; ++i) M = fmaxf(M, scratch.ml[first + i * step].x);
+        float L = 0.0f, acc[kHeadMax / 32] = {};
+#pragma unroll 4
+        for (int i = 0; i < it.n_parts; ++i) {
+            const size_t w = first + i * step;
+            const float2 ml = scratch.ml[w];
+            const float k = M == -INFINITY ? 0.0f : ex2(ml.x - M);
+            L = __fmaf_rn(ml.y, k, L);
+#pragma unroll
+            for (int x = 0; x < kHeadMax / 32; ++x)
+                if (lane + 32 * x < p.head) acc[x] = __fmaf_rn(scratch.o[w * p.head + lane + 32 * x], k, acc[x]);
+        }
+        const int mr = it.row + r, tok = mr / p.group;
+        const size_t at = ((size_t)(sq.row0 + tok) * p.heads + (size_t)j * p.group + (mr - tok * p.group)) * p.head;
+#pragma unroll
+        for (int x = 0; x < kHeadMax / 32; ++x)
+            if (lane + 32 * x < p.head) out[at + lane + 32 * x] = acc[x] / L;
+    }
+}
+
+template <int D, bool F32>
+cudaError_t launch(const PagesView &p, int layer, const StepSeq *seqs, const AttnItem *items, int n_items,
+                   const AttnScratch &scratch, const float *q, float *out, int *err, cudaStream_t s) {
+    static bool attr_done[64] = {false};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) dev = 0;
+    if (!attr_done[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(k_pages_prompt<D, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (int)Shape<D, F32>::Smem);
+        if (e != cudaSuccess) return e;
+        attr_done[dev] = true;
+    }
+    k_pages_prompt<D, F32><<<(unsigned)p.kv_heads * (unsigned)n_items, kPromptThreads, Shape<D, F32>::Smem, s>>>(
+        p, layer, seqs, items, scratch, q, out, err);
+    count_launch();
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_pages_prompt(const PagesView &p, int layer, const StepSeq *seqs, const AttnItem *items, int n_items,
+                                bool split, const AttnScratch &scratch, const float *q, float *out, int *err,
+                                cudaStream_t s) {
+    if (n_items == 0) return cudaSuccess;
+    const cudaError_t e =
+        p.head <= 64 ? (p.f32 ? launch<64, true>(p, layer, seqs, items, n_items, scratch, q, out, err, s)
+                              : launch<64, false>(p, layer, seqs, items, n_items, scratch, q, out, err, s))
+                     : (p.f32 ? launch<128, true>(p, layer, seqs, items, n_items, scratch, q, out, err, s)
+                              : launch<128, false>(p, layer, seqs, items, n_items, scratch, q, out, err, s));
+    if (e != cudaSuccess || !split) return e;
+    k_pages_join<<<dim3((unsigned)p.kv_heads * (unsigned)n_items, 8), 128, 0, s>>>(p, seqs, items, scratch, out);
+    count_launch();
+    return cudaGetLastError();
+}
+
+}  // namespace krt

@@ -57,6 +57,7 @@ struct Shape {
     static constexpr int Slots = D == 64 ? (F32 ? 4 : 6) : 3;
     static constexpr int QTile = 2 * (D / 64) * 128 * 128;  // both halves of 128 rows
     static constexpr size_t Smem = 2 * (size_t)QTile + (size_t)Slots * Slot + 1024;
+    static constexpr int Wide = D == 64 ? 32 : 16;  // columns a softmax thread takes at a time
     static constexpr int Region = Keys + D;  // TMEM columns of a query tile: scores / weights, sum of V
 };
 
@@ -98,15 +99,78 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-        : "memory");
+// W columns of this warp's lanes, one lane per thread.  A load is in flight until
+// the wait, which v passes through, so that no use of it moves ahead.
+template <int W>
+struct Tmem;
+template <>
+struct Tmem<16> {
+    using V = uint32_t[16];
+    static __device__ __forceinline__ void load(uint32_t taddr, V &v) {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+                       "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+                       "=r"(v[14]), "=r"(v[15])
+                     : "r"(taddr));
+    }
+    static __device__ __forceinline__ void wait(V &v) {
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]),
+                       "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]),
+                       "+r"(v[14]), "+r"(v[15])::"memory");
+    }
+    static __device__ __forceinline__ void store(uint32_t taddr, const V &v) {
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+                     "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                     "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+                     "r"(v[15])
+                     : "memory");
+    }
+};
+template <>
+struct Tmem<32> {
+    using V = uint32_t[32];
+    static __device__ __forceinline__ void load(uint32_t taddr, V &v) {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+                       "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+                       "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
+                       "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]),
+                       "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                     : "r"(taddr));
+    }
+    static __device__ __forceinline__ void wait(V &v) {
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]),
+                       "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]),
+                       "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]),
+                       "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]),
+                       "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])::"memory");
+    }
+    static __device__ __forceinline__ void store(uint32_t taddr, const V &v) {
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+                     "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                     "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+                     "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
+                     "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+                     "r"(v[29]), "r"(v[30]), "r"(v[31])
+                     : "memory");
+    }
+};
+
+// Calls use(c, v) for columns c .. c + W - 1 of N from taddr on, each load in
+// flight while the columns before it are used.
+template <int N, int W, class F>
+__device__ __forceinline__ void tmem_each(uint32_t taddr, F &&use) {
+    uint32_t v[2][W];
+    Tmem<W>::load(taddr, v[0]);
+#pragma unroll
+    for (int c = 0; c < N; c += W) {
+        uint32_t(&now)[W] = v[(c / W) & 1];
+        Tmem<W>::wait(now);
+        if (c + W < N) Tmem<W>::load(taddr + (uint32_t)(c + W), v[((c / W) & 1) ^ 1]);
+        use(c, now);
+    }
 }
 
 __device__ __forceinline__ uint32_t pack_half(float a, float b) {
@@ -167,12 +231,17 @@ __device__ __forceinline__ bool loader_or(bool p) {
     return r != 0;
 }
 
+template <int T>
+struct Tile {  // a query tile, known at compile time
+    __device__ __forceinline__ constexpr operator int() const { return T; }
+};
+
 template <int D, bool F32>
 __global__ void __launch_bounds__(kPromptThreads, 1)
     k_pages_prompt(PagesView p, int layer, const StepSeq *__restrict__ seqs, const AttnItem *__restrict__ items,
                    AttnScratch scratch, const float *__restrict__ q, float *__restrict__ out, int *err) {
     using S = Shape<D, F32>;
-    constexpr int Keys = S::Keys;
+    constexpr int Keys = S::Keys, W = S::Wide;
     extern __shared__ unsigned char raw_smem[];
     __shared__ uint64_t slot_full[S::Slots], slot_empty[S::Slots], s_full[2], p_full[2], q_full, done;
     __shared__ uint32_t s_tmem, s_red[2][4][2];
@@ -211,22 +280,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     const AttnItem it = items[item];
     const StepSeq sq = seqs[it.seq];
     const int32_t *table = p.table + (size_t)sq.slot * p.max_pages;
-    // key tiles of the two query tiles: up to the last position any row sees
-    int n_tiles[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    // key tiles of a query tile: up to the last position any of its rows sees
+    const auto tiles_of = [&](int t) {
         const int last = min(it.rows, 128 * (t + 1)) - 1;
         const int seen = min(it.hi, sq.ctx + (it.row + last) / p.group + 1) - it.lo;
-        n_tiles[t] = last < 128 * t || seen <= 0 ? 0 : (seen + Keys - 1) / Keys;
-    }
-    const int n = max(n_tiles[0], n_tiles[1]);
+        return last < 128 * t || seen <= 0 ? 0 : (seen + Keys - 1) / Keys;
+    };
+    const int n0 = tiles_of(0), n1 = tiles_of(1), n = max(n0, n1);
 
-    const auto wait = [&](uint64_t *bar, int phase) {
-        if (mbar_try_wait(bar, (uint32_t)phase & 1u)) return true;
-        const long long t0 = clock64();
-        while (!mbar_try_wait(bar, (uint32_t)phase & 1u)) {
+    const auto wait = [&](uint64_t *bar, uint32_t parity) {
+        if (mbar_try_wait(bar, parity)) return true;
+        const uint32_t t0 = (uint32_t)clock();
+        while (!mbar_try_wait(bar, parity)) {
             if (*abort_flag) return false;
-            if (clock64() - t0 > (1ll << 31)) {
+            if ((uint32_t)clock() - t0 > 1u << 31) {  // about a second
                 if (err) atomicOr(err, ERR_TIMEOUT);
                 *abort_flag = 1;
                 return false;
@@ -237,7 +304,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 
     if (warp < 8) {
         // ---- a thread per query row -----------------------------------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
         const int t = warp >> 2, r = threadIdx.x;  // r = 128 t + row of the tile
         const bool live = r < it.rows;
         const int m_row = it.row + (live ? r : 0), token = m_row / p.group;
@@ -292,37 +359,31 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const uint32_t s_at = tmem + lanes + (uint32_t)(t * S::Region), o_at = s_at + Keys;
         const auto flush = [&](int tile) {  // the tile's sum of V into the registers
             const float vs = s_vscale[tile & (kScaleRing - 1)];
+            tmem_each<D, W>(o_at, [&](int c, uint32_t(&v)[W]) {
 #pragma unroll
-            for (int c = 0; c < D; c += 32) {
-                uint32_t v[32];
-                tmem_ld32(o_at + (uint32_t)c, v);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) acc[c + i] = __fmaf_rn(__uint_as_float(v[i]), vs, acc[c + i]);
-            }
+                for (int i = 0; i < W; ++i) acc[c + i] = __fmaf_rn(__uint_as_float(v[i]), vs, acc[c + i]);
+            });
         };
         bool ok = true;
-        const int mine = n_tiles[t];
+        const int mine = t ? n1 : n0;
         for (int tile = 0; tile < mine; ++tile) {
-            ok = __all_sync(0xffffffffu, wait(&s_full[t], tile));
+            ok = __all_sync(0xffffffffu, wait(&s_full[t], (uint32_t)tile & 1u));
             if (!ok) break;
             tc_fence_after();
             const int rem = limit - (it.lo + tile * Keys);  // the tile's keys this row sees
             const bool masked = __any_sync(0xffffffffu, rem < Keys);
             const float ks = sc * s_kscale[tile & (kScaleRing - 1)];
-            float mx = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < Keys; c += 32) {
-                uint32_t v[32];
-                tmem_ld32(s_at + (uint32_t)c, v);
+            float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tmem_each<Keys, W>(s_at, [&](int c, uint32_t(&v)[W]) {
                 if (masked) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (c + i < rem) mx = fmaxf(mx, __uint_as_float(v[i]));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(v[i]));
+                    for (int i = 0; i < W; ++i)
+                        if (c + i >= rem) v[i] = 0xff800000u;  // -inf
                 }
-            }
+#pragma unroll
+                for (int i = 0; i < W; ++i) part[i & 3] = fmaxf(part[i & 3], __uint_as_float(v[i]));
+            });
+            const float mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
             if (tile) flush(tile - 1);
             const float mn = fmaxf(m, mx * ks);
             if (tile && __any_sync(0xffffffffu, mn > m)) {
@@ -334,40 +395,36 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             m = mn;
             // weights times 2^14: the halves of small ones stay normal numbers
             const float bias = 14.0f - (m == -INFINITY ? 0.0f : m);
-            float sum = 0.0f;
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            tmem_each<Keys, W>(s_at, [&](int c, uint32_t(&v)[W]) {
 #pragma unroll
-            for (int c = 0; c < Keys; c += 32) {
-                uint32_t v[32];
-                tmem_ld32(s_at + (uint32_t)c, v);
-                float w[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) w[i] = ex2(__fmaf_rn(__uint_as_float(v[i]), ks, bias));
+                for (int i = 0; i < W; ++i) v[i] = __float_as_uint(ex2(__fmaf_rn(__uint_as_float(v[i]), ks, bias)));
                 if (masked) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (c + i >= rem) w[i] = 0.0f;
+                    for (int i = 0; i < W; ++i)
+                        if (c + i >= rem) v[i] = 0u;
                 }
-                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                // in place: W / 2 columns of the halves hi, W / 2 of lo
+                uint32_t h[W];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) part[i & 3] += w[i];
-                sum += (part[0] + part[1]) + (part[2] + part[3]);
-                // in place: 16 columns of the halves hi, 16 of lo
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    v[i] = pack_half(w[2 * i], w[2 * i + 1]);
-                    const float2 f = unpack_half(v[i]);
-                    v[16 + i] = pack_half(w[2 * i] - f.x, w[2 * i + 1] - f.y);
+                for (int i = 0; i < W / 2; ++i) {
+                    const float a = __uint_as_float(v[2 * i]), b = __uint_as_float(v[2 * i + 1]);
+                    sum[(2 * i) & 3] += a;
+                    sum[(2 * i + 1) & 3] += b;
+                    h[i] = pack_half(a, b);
+                    const float2 f = unpack_half(h[i]);
+                    h[W / 2 + i] = pack_half(a - f.x, b - f.y);
                 }
-                tmem_st32(s_at + (uint32_t)c, v);
-            }
-            l += sum;
+                Tmem<W>::store(s_at + (uint32_t)c, h);
+            });
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[t]);
         }
         if (ok && mine) {
-            ok = __all_sync(0xffffffffu, wait(&s_full[t], mine));
+            ok = __all_sync(0xffffffffu, wait(&s_full[t], (uint32_t)mine & 1u));
             tc_fence_after();
             if (ok) flush(mine - 1);
         }
@@ -411,30 +468,35 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const size_t page_stride = (size_t)p.kv_heads * ((size_t)p.head << p.page_shift);
         const size_t v_off = page_elem(p, layer, 1, 0, j) - page_elem(p, layer, 0, 0, j);
         const size_t k_base = page_elem(p, layer, 0, 0, j) + 8 * chunk;
-        int pages = 0;  // lane i: the page of positions 16 i .. of the tile
-        for (int i = 0; i < 2 * n; ++i) {
-            const int key0 = it.lo + (i >> 1) * Keys, slot = i % S::Slots;
-            if (!(i & 1)) {
-                const int pos = key0 + 16 * lane;
-                pages = lane < Keys / 16 && pos < it.hi ? __ldg(table + (pos >> p.page_shift)) : 0;
+        // lane i: the page of positions 16 i .. of a tile; kept one tile ahead
+        const auto page_ids = [&](int tile) {
+            const int pos = it.lo + tile * Keys + 16 * lane;
+            return lane < Keys / 16 && pos < it.hi ? __ldg(table + (pos >> p.page_shift)) : 0;
+        };
+        int pages = page_ids(0), pages_next = 0;
+        uint4 v[Loads * (F32 ? 2 : 1)];
+        const auto load = [&](int i, int k, int ids) {  // rows k * Step .. of the i-th tile of the ring
+            const int pos = it.lo + (i >> 1) * Keys + k * Step + row;
+            const int page = __shfl_sync(0xffffffffu, ids, k * Step / 16);
+            const size_t e = k_base + ((i & 1) ? v_off : 0) + (size_t)page * page_stride + (size_t)(pos & page_mask) * p.head;
+            const bool in = have && pos < it.hi;
+            const uint4 zero = make_uint4(0, 0, 0, 0);
+            if constexpr (F32) {
+                const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const float *>(p.kv) + e);
+                v[2 * k] = in ? __ldg(src) : zero;
+                v[2 * k + 1] = in ? __ldg(src + 1) : zero;
+            } else {
+                v[k] = in ? __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.kv) + e)) : zero;
             }
-            const size_t tile_base = k_base + ((i & 1) ? v_off : 0);
-            uint4 v[Loads * (F32 ? 2 : 1)];
+        };
+        if (n > 0) {
 #pragma unroll
-            for (int k = 0; k < Loads; ++k) {
-                const int pos = key0 + k * Step + row;
-                const int page = __shfl_sync(0xffffffffu, pages, k * Step / 16);
-                const size_t e = tile_base + (size_t)page * page_stride + (size_t)(pos & page_mask) * p.head;
-                const bool in = have && pos < it.hi;
-                const uint4 zero = make_uint4(0, 0, 0, 0);
-                if constexpr (F32) {
-                    const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const float *>(p.kv) + e);
-                    v[2 * k] = in ? __ldg(src) : zero;
-                    v[2 * k + 1] = in ? __ldg(src + 1) : zero;
-                } else {
-                    v[k] = in ? __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.kv) + e)) : zero;
-                }
-            }
+            for (int k = 0; k < Loads; ++k) load(0, k, pages);
+        }
+        int slot = 0;
+        uint32_t freed = 1;  // parity of the slot's last use; the first round finds every slot free
+        for (int i = 0; i < 2 * n; ++i) {
+            if (!(i & 1)) pages_next = page_ids((i >> 1) + 1);
             // the tile's largest magnitude, and the smallest of the chunks'
             uint32_t most = 0, least = 0xffffffffu;
 #pragma unroll
@@ -462,7 +524,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 red[warp - 8][0] = most;
                 red[warp - 8][1] = least;
             }
-            const bool ok = i < S::Slots || wait(&slot_empty[slot], i / S::Slots - 1);
+            const bool ok = wait(&slot_empty[slot], freed);
             if (loader_or(!ok)) break;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
@@ -475,96 +537,117 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 ((i & 1) ? s_vscale : s_kscale)[(i >> 1) & (kScaleRing - 1)] = down_scale(up);
             }
             const uint32_t dst = slots + (uint32_t)slot * S::Slot + (uint32_t)(chunk >> 3) * S::Sub;
+            // a chunk's registers take the next tile's as soon as it is stored
+            const bool more = i + 1 < 2 * n;
+            const int ids = (i & 1) ? pages_next : pages;
 #pragma unroll
             for (int k = 0; k < Loads; ++k) {
-                float x[8];
-                if constexpr (F32) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float((&v[2 * k + (e >> 2)].x)[e & 3]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t u = (&v[k].x)[e];
-                        x[2 * e] = __uint_as_float(u << 16);
-                        x[2 * e + 1] = __uint_as_float(u & 0xffff0000u);
-                    }
-                }
                 uint4 hi, lo;
-                halves<F32>(x, up, hi, lo);
+                if constexpr (F32) {
+                    const float x[8] = {__uint_as_float(v[2 * k].x),     __uint_as_float(v[2 * k].y),
+                                        __uint_as_float(v[2 * k].z),     __uint_as_float(v[2 * k].w),
+                                        __uint_as_float(v[2 * k + 1].x), __uint_as_float(v[2 * k + 1].y),
+                                        __uint_as_float(v[2 * k + 1].z), __uint_as_float(v[2 * k + 1].w)};
+                    halves<true>(x, up, hi, lo);
+                } else {
+                    const float x[8] = {__uint_as_float(v[k].x << 16), __uint_as_float(v[k].x & 0xffff0000u),
+                                        __uint_as_float(v[k].y << 16), __uint_as_float(v[k].y & 0xffff0000u),
+                                        __uint_as_float(v[k].z << 16), __uint_as_float(v[k].z & 0xffff0000u),
+                                        __uint_as_float(v[k].w << 16), __uint_as_float(v[k].w & 0xffff0000u)};
+                    halves<false>(x, up, hi, lo);
+                }
                 const uint32_t o = dst + swizzled(k * Step + row, chunk & 7);
                 store_shared(o, hi);
                 if (F32) store_shared(o + (D / 64) * S::Sub, lo);
+                if (more) load(i + 1, k, ids);
             }
+            if (i & 1) pages = pages_next;
             fence_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&slot_full[slot]);
+            if (++slot == S::Slots) slot = 0, freed ^= 1;
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
-        if (warp == 12 && lane == 0) {
-            // ---- the MMAs ---------------------------------------------------------
-            const auto scores = [&](int t, int tile) {  // S = (q_hi + q_lo) K^T
-                const uint32_t k = slots + (uint32_t)(2 * tile % S::Slots) * S::Slot, a = base + (uint32_t)t * S::QTile;
-                uint32_t more = 0;
-#pragma unroll 1
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 12) {
+            // ---- the MMAs: the warp waits as one, one lane issues ---------------------------------------------------------
+            // addresses in descriptors are in units of 16 bytes: offsets add
+            const uint64_t qd = sw128_desc(base), kd = sw128_desc(slots), vd = mn_desc(slots, S::Sub);
+            const auto scores = [&](auto t, int slot) {  // S = (q_hi + q_lo) K^T
+                if (!elect_one()) return;
+                const uint64_t a = qd + (uint64_t)(t * S::QTile >> 4), k = kd + (uint64_t)(slot * (S::Slot >> 4));
+#pragma unroll
                 for (int x = 0; x < S::Parts + 1; ++x) {  // q_hi K_hi, q_lo K_hi, q_hi K_lo
-                    const uint32_t qa = a + (x == 1 ? (D / 64) * 16384 : 0), kb = k + (x == 2 ? (D / 64) * S::Sub : 0);
+                    const int qo = x == 1 ? (D / 64) * 16384 : 0, ko = x == 2 ? (D / 64) * S::Sub : 0;
 #pragma unroll
-                    for (int d = 0; d < D / 16; ++d) {
-                        mma_ss(tmem + (uint32_t)(t * S::Region), sw128_desc(qa + (d >> 2) * 16384 + (d & 3) * 32),
-                               sw128_desc(kb + (d >> 2) * S::Sub + (d & 3) * 32), idesc<Keys, false>(), more);
-                        more = 1;
-                    }
+                    for (int d = 0; d < D / 16; ++d)
+                        mma_ss(tmem + t * S::Region, a + ((qo + (d >> 2) * 16384 + (d & 3) * 32) >> 4),
+                               k + ((ko + (d >> 2) * S::Sub + (d & 3) * 32) >> 4), idesc<Keys, false>(), x | d);
                 }
             };
-            const auto values = [&](int t, int tile) {  // O = (w_hi + w_lo) V
-                const uint32_t v = slots + (uint32_t)((2 * tile + 1) % S::Slots) * S::Slot;
-                const uint32_t w = tmem + (uint32_t)(t * S::Region);
-                uint32_t more = 0;
-#pragma unroll 1
+            const auto values = [&](auto t, int slot) {  // O = (w_hi + w_lo) V
+                if (!elect_one()) return;
+                const uint64_t v = vd + (uint64_t)(slot * (S::Slot >> 4));
+                const uint32_t w = tmem + t * S::Region;
+#pragma unroll
                 for (int x = 0; x < S::Parts + 1; ++x) {  // w_hi V_hi, w_lo V_hi, w_hi V_lo
-                    const uint32_t vb = v + (x == 2 ? (D / 64) * S::Sub : 0);
+                    const int vo = x == 2 ? (D / 64) * S::Sub : 0;
 #pragma unroll
-                    for (int k = 0; k < Keys / 16; ++k) {
-                        mma_ts(w + Keys, w + (uint32_t)((k >> 1) * 32 + (x == 1 ? 16 : 0) + (k & 1) * 8),
-                               mn_desc(vb + (uint32_t)k * 2048, S::Sub), idesc<D, true>(), more);
-                        more = 1;
-                    }
+                    for (int k = 0; k < Keys / 16; ++k)
+                        mma_ts(w + Keys, w + k * 16 / W * W + k * 16 % W / 2 + (x == 1 ? W / 2 : 0), v + ((vo + k * 2048) >> 4),
+                               idesc<D, true>(), x | k);
                 }
             };
-            const auto full = [&](int i) { return wait(&slot_full[i % S::Slots], i / S::Slots); };
-            bool ok = wait(&q_full, 0) && (n == 0 || full(0));
+            const auto commit = [&](uint64_t *bar) {
+                if (elect_one()) mma_commit(bar);
+            };
+            const auto wait_all = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+            struct Place {  // of the K or V tiles in the ring
+                int slot;
+                uint32_t parity;
+                __device__ __forceinline__ void next() {
+                    slot += 2;
+                    if (slot >= S::Slots) slot -= S::Slots, parity ^= 1;
+                }
+            };
+            Place kp{0, 0}, vp{1, 0};
+            bool ok = wait_all(&q_full, 0) && (n == 0 || wait_all(&slot_full[0], 0));
             if (ok && n > 0) {
                 tc_fence_after();
-                for (int t = 0; t < 2; ++t)
-                    if (n_tiles[t] > 0) {
-                        scores(t, 0);
-                        mma_commit(&s_full[t]);
-                    }
-                mma_commit(&slot_empty[0]);
+                if (n0 > 0) {
+                    scores(Tile<0>{}, 0);
+                    commit(&s_full[0]);
+                }
+                if (n1 > 0) {
+                    scores(Tile<1>{}, 0);
+                    commit(&s_full[1]);
+                }
+                commit(&slot_empty[0]);
+                kp.next();
             }
             for (int tile = 0; ok && tile < n; ++tile) {
-                for (int t = 0; ok && t < 2; ++t) {
-                    if (tile >= n_tiles[t]) continue;
-                    ok = full(2 * tile + 1) && wait(&p_full[t], tile);
-                    if (!ok) break;
+                const auto turn = [&](auto t, int mine) {
+                    if (tile >= mine) return true;
+                    if (!wait_all(&slot_full[vp.slot], vp.parity) || !wait_all(&p_full[t], (uint32_t)tile & 1u)) return false;
                     tc_fence_after();
-                    values(t, tile);
-                    if (tile + 1 < n_tiles[t]) {
-                        ok = full(2 * tile + 2);
-                        if (!ok) break;
+                    values(t, vp.slot);
+                    if (tile + 1 < mine) {
+                        if (!wait_all(&slot_full[kp.slot], kp.parity)) return false;
                         tc_fence_after();
-                        scores(t, tile + 1);
+                        scores(t, kp.slot);
                     }
-                    mma_commit(&s_full[t]);
-                }
+                    commit(&s_full[t]);
+                    return true;
+                };
+                ok = turn(Tile<0>{}, n0) && turn(Tile<1>{}, n1);
                 if (!ok) break;
-                mma_commit(&slot_empty[(2 * tile + 1) % S::Slots]);
-                if (tile + 1 < n) mma_commit(&slot_empty[(2 * tile + 2) % S::Slots]);
+                commit(&slot_empty[vp.slot]);
+                if (tile + 1 < n) commit(&slot_empty[kp.slot]);
+                vp.next();
+                kp.next();
             }
-            mma_commit(&done);  // every MMA issued, finished loop or not
+            commit(&done);  // every MMA issued, finished loop or not
         }
-        __syncwarp();
     }
     tc_fence_before();
     __syncthreads();

@@ -68,35 +68,44 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // Instruction descriptor of kind::f16: D f32 (bits 4-5 = 1), A and B fp16 (bits
-// 7-9, 10-12 = 0), A K-major, B K-major or (bit 16) MN-major, N / 8 at bits
-// 17-22, M / 16 at bits 24-28.
+// 7-9, 10-12 = 0), A or B negated (bits 13, 14), A K-major, B K-major or (bit
+// 16) MN-major, N / 8 at bits 17-22, M / 16 at bits 24-28.
 template <int N, bool MnMajor>
-__host__ __device__ constexpr uint32_t idesc() {
-    return (1u << 4) | (MnMajor ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+__host__ __device__ constexpr uint32_t idesc(bool neg_a, bool neg_b) {
+    return (1u << 4) | (neg_a ? 1u << 13 : 0u) | (neg_b ? 1u << 14 : 0u) | (MnMajor ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
-// Descriptor of an MN-major tile [K rows][64 of N per sub-tile], 128-byte
-// swizzled: 8-row groups of K 1 KB apart (stride byte offset), 64-wide groups
-// of N `sub` bytes apart (leading byte offset).
-__device__ __forceinline__ uint64_t mn_desc(uint32_t saddr, uint32_t sub) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((sub >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
+// Lower words of the descriptors of a 128-byte swizzled tile: K-major (the
+// leading byte offset unused), and MN-major [K rows][64 of N per sub-tile] with
+// 8-row groups of K 1 KB apart (the stride byte offset, as in K-major) and
+// 64-wide groups of N `sub` bytes apart (leading byte offset).
+__device__ __forceinline__ uint32_t k_desc(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t mn_desc(uint32_t saddr, uint32_t sub) { return (saddr >> 4) | ((sub >> 4) << 16); }
+
+// The upper word of both descriptors; the lower one holds the address, in units
+// of 16 bytes, to which offsets are added.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
 
 // D += A B with A from shared memory, or from TMEM.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t desc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(desc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(desc), "r"(accumulate), "r"(kDescHigh)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t desc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(desc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(desc), "r"(accumulate), "r"(kDescHigh)
         : "memory");
+}
+// Keeps address arithmetic next to its use: hoisted out of the loop, the
+// operands of every MMA would each hold a register.
+__device__ __forceinline__ uint32_t here(uint32_t x) {
+    asm volatile("" : "+r"(x));
+    return x;
 }
 
 // W columns of this warp's lanes, one lane per thread.  A load is in flight until
@@ -173,12 +182,55 @@ __device__ __forceinline__ void tmem_each(uint32_t taddr, F &&use) {
     }
 }
 
-__device__ __forceinline__ uint32_t pack_half(float a, float b) {
-    const __half2 v = __floats2half2_rn(a, b);
+// Pairs at a time: sm_100 adds and multiplies two f32 in one instruction, and
+// takes an fp16 half from an f32 in one.
+struct F2 {
+    float x, y;
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 d;
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 d;
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\t"
+        "mov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 d;
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\t"
+        "mov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ F2 pair(uint32_t a, uint32_t b) { return {__uint_as_float(a), __uint_as_float(b)}; }
+__device__ __forceinline__ F2 both(float a) { return {a, a}; }
+
+__device__ __forceinline__ uint32_t pack_half(F2 a) {
+    const __half2 v = __floats2half2_rn(a.x, a.y);
     return *reinterpret_cast<const uint32_t *>(&v);
 }
-__device__ __forceinline__ float2 unpack_half(uint32_t v) {
-    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+// A pair as fp16: hi, and what hi has too much of it, -lo (the MMAs negate it).
+__device__ __forceinline__ void split_half(F2 a, uint32_t &hi, uint32_t &neg_lo) {
+    hi = pack_half(a);
+    F2 d;
+    asm("{\n\t.reg .f16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.f16 %0, l, %3;\n\tsub.rn.f32.f16 %1, h, %4;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "r"(hi), "f"(a.x), "f"(a.y));
+    neg_lo = pack_half(d);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 // The power of two that brings a magnitude with these bits to [2^13, 2^14), and
@@ -203,21 +255,28 @@ __device__ __forceinline__ void store_shared(uint32_t addr, uint4 v) {
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Eight f32 values times s as fp16: the halves hi and, if wanted, lo.
-template <bool Lo>
-__device__ __forceinline__ void halves(const float (&x)[8], float s, uint4 &hi, uint4 &lo) {
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float a = x[2 * i] * s, b = x[2 * i + 1] * s;
-        h[i] = pack_half(a, b);
-        if (Lo) {
-            const float2 f = unpack_half(h[i]);
-            l[i] = pack_half(a - f.x, b - f.y);
-        }
-    }
-    hi = make_uint4(h[0], h[1], h[2], h[3]);
-    if (Lo) lo = make_uint4(l[0], l[1], l[2], l[3]);
+// Eight f32 values times s as fp16 halves hi and -lo.
+__device__ __forceinline__ void halves(const float4 &a, const float4 &b, float s, uint4 &hi, uint4 &lo) {
+    split_half(mul2({a.x, a.y}, both(s)), hi.x, lo.x);
+    split_half(mul2({a.z, a.w}, both(s)), hi.y, lo.y);
+    split_half(mul2({b.x, b.y}, both(s)), hi.z, lo.z);
+    split_half(mul2({b.z, b.w}, both(s)), hi.w, lo.w);
+}
+// A pair of bf16 times a power of two (exact) as fp16.
+__device__ __forceinline__ uint32_t to_half(uint32_t u, __nv_bfloat162 s) {
+    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&u), s);
+    u = *reinterpret_cast<const uint32_t *>(&v);
+    return pack_half(pair(u << 16, u & 0xffff0000u));
+}
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t min_u16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("min.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
 }
 
 // Barrier of the loader's 128 threads that also says whether any of them has p.
@@ -304,7 +363,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 
     if (warp < 8) {
         // ---- a thread per query row -----------------------------------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         const int t = warp >> 2, r = threadIdx.x;  // r = 128 t + row of the tile
         const bool live = r < it.rows;
         const int m_row = it.row + (live ? r : 0), token = m_row / p.group;
@@ -334,14 +393,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             const uint32_t tile = base + (uint32_t)t * S::QTile;
 #pragma unroll 2
             for (int c = 0; c < D / 8; ++c) {
-                float x[8] = {};
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
                 if (live && c < chunks) {
-                    const float4 a = __ldg(src + 2 * c), b = __ldg(src + 2 * c + 1);
-                    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-                    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+                    x = __ldg(src + 2 * c);
+                    y = __ldg(src + 2 * c + 1);
                 }
                 uint4 hi, lo;
-                halves<true>(x, up, hi, lo);
+                halves(x, y, up, hi, lo);
                 const uint32_t o = tile + (uint32_t)(c >> 3) * 16384 + swizzled(r & 127, c & 7);
                 store_shared(o, hi);
                 store_shared(o + (D / 64) * 16384, lo);
@@ -351,9 +409,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             if (lane == 0) mbar_arrive(&q_full);
         }
 
-        float acc[D];
+        F2 acc[D / 2];
 #pragma unroll
-        for (int d = 0; d < D; ++d) acc[d] = 0.0f;
+        for (int d = 0; d < D / 2; ++d) acc[d] = both(0.0f);
         float m = -INFINITY, l = 0.0f;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t s_at = tmem + lanes + (uint32_t)(t * S::Region), o_at = s_at + Keys;
@@ -361,7 +419,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             const float vs = s_vscale[tile & (kScaleRing - 1)];
             tmem_each<D, W>(o_at, [&](int c, uint32_t(&v)[W]) {
 #pragma unroll
-                for (int i = 0; i < W; ++i) acc[c + i] = __fmaf_rn(__uint_as_float(v[i]), vs, acc[c + i]);
+                for (int i = 0; i < W / 2; ++i)
+                    acc[c / 2 + i] = fma2(pair(v[2 * i], v[2 * i + 1]), both(vs), acc[c / 2 + i]);
             });
         };
         bool ok = true;
@@ -381,7 +440,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                         if (c + i >= rem) v[i] = 0xff800000u;  // -inf
                 }
 #pragma unroll
-                for (int i = 0; i < W; ++i) part[i & 3] = fmaxf(part[i & 3], __uint_as_float(v[i]));
+                for (int i = 0; i < W; i += 2)
+                    part[i / 2 & 3] = max3(part[i / 2 & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
             });
             const float mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
             if (tile) flush(tile - 1);
@@ -390,34 +450,29 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 const float keep = mn == -INFINITY ? 0.0f : ex2(m - mn);
                 l *= keep;
 #pragma unroll
-                for (int d = 0; d < D; ++d) acc[d] *= keep;
+                for (int d = 0; d < D / 2; ++d) acc[d] = mul2(acc[d], both(keep));
             }
             m = mn;
             // weights times 2^14: the halves of small ones stay normal numbers
             const float bias = 14.0f - (m == -INFINITY ? 0.0f : m);
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            F2 sum[2] = {both(0.0f), both(0.0f)};
             tmem_each<Keys, W>(s_at, [&](int c, uint32_t(&v)[W]) {
-#pragma unroll
-                for (int i = 0; i < W; ++i) v[i] = __float_as_uint(ex2(__fmaf_rn(__uint_as_float(v[i]), ks, bias)));
-                if (masked) {
-#pragma unroll
-                    for (int i = 0; i < W; ++i)
-                        if (c + i >= rem) v[i] = 0u;
-                }
-                // in place: W / 2 columns of the halves hi, W / 2 of lo
+                // in place: W / 2 columns of the halves hi, W / 2 of -lo
                 uint32_t h[W];
 #pragma unroll
                 for (int i = 0; i < W / 2; ++i) {
-                    const float a = __uint_as_float(v[2 * i]), b = __uint_as_float(v[2 * i + 1]);
-                    sum[(2 * i) & 3] += a;
-                    sum[(2 * i + 1) & 3] += b;
-                    h[i] = pack_half(a, b);
-                    const float2 f = unpack_half(h[i]);
-                    h[W / 2 + i] = pack_half(a - f.x, b - f.y);
+                    const F2 x = fma2(pair(v[2 * i], v[2 * i + 1]), both(ks), both(bias));
+                    F2 w{ex2(x.x), ex2(x.y)};
+                    if (masked) {
+                        if (c + 2 * i >= rem) w.x = 0.0f;
+                        if (c + 2 * i + 1 >= rem) w.y = 0.0f;
+                    }
+                    sum[i & 1] = add2(sum[i & 1], w);
+                    split_half(w, h[i], h[W / 2 + i]);
                 }
                 Tmem<W>::store(s_at + (uint32_t)c, h);
             });
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
@@ -431,14 +486,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (ok) {
             bool fine = isfinite(l) && !*(volatile int *)&s_wild;
 #pragma unroll
-            for (int d = 0; d < D; ++d) fine = fine && isfinite(acc[d]);
+            for (int d = 0; d < D / 2; ++d) fine = fine && isfinite(acc[d].x) && isfinite(acc[d].y);
             const size_t part = ((size_t)item * p.kv_heads + j) * kRows + r;
             if (live && fine) {
                 const float f = it.n_parts == 1 ? 1.0f / l : 0x1p-14f;
                 float4 *dst = reinterpret_cast<float4 *>(it.n_parts == 1 ? out + at : scratch.o + part * p.head);
 #pragma unroll
-                for (int d = 0; d < D; d += 4)
-                    if (d < p.head) dst[d / 4] = make_float4(acc[d] * f, acc[d + 1] * f, acc[d + 2] * f, acc[d + 3] * f);
+                for (int d = 0; d < D / 2; d += 2)
+                    if (2 * d < p.head)
+                        dst[d / 2] = make_float4(acc[d].x * f, acc[d].y * f, acc[d + 1].x * f, acc[d + 1].y * f);
                 if (it.n_parts > 1) scratch.ml[part] = make_float2(m, l * 0x1p-14f);
             }
             unsigned again = __ballot_sync(0xffffffffu, live && !fine);
@@ -463,59 +519,68 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         constexpr int PerRow = D / 8, Step = 128 / PerRow;  // eight-element chunks of a row, rows of a step
         constexpr int Loads = Keys / Step;
         const int tid = threadIdx.x - 256, chunk = tid % PerRow, row = tid / PerRow;
-        const bool have = chunk < (p.head >> 3);
+        constexpr uint32_t Size = F32 ? 4 : 2;
         const int page_mask = (1 << p.page_shift) - 1;
-        const size_t page_stride = (size_t)p.kv_heads * ((size_t)p.head << p.page_shift);
-        const size_t v_off = page_elem(p, layer, 1, 0, j) - page_elem(p, layer, 0, 0, j);
-        const size_t k_base = page_elem(p, layer, 0, 0, j) + 8 * chunk;
-        // lane i: the page of positions 16 i .. of a tile; kept one tile ahead
-        const auto page_ids = [&](int tile) {
+        const uint32_t row_bytes = (uint32_t)p.head * Size;
+        const size_t page_bytes = (size_t)p.kv_heads * ((size_t)row_bytes << p.page_shift);
+        const char *k_src = static_cast<const char *>(p.kv) + (page_elem(p, layer, 0, 0, j) + 8 * chunk) * Size +
+                            (size_t)row * row_bytes;
+        const char *v_src = k_src + (page_elem(p, layer, 1, 0, j) - page_elem(p, layer, 0, 0, j)) * Size;
+        // lane i: where positions 16 i .. of a tile lie; kept one tile ahead
+        const auto places = [&](int tile) {
             const int pos = it.lo + tile * Keys + 16 * lane;
-            return lane < Keys / 16 && pos < it.hi ? __ldg(table + (pos >> p.page_shift)) : 0;
+            if (lane >= Keys / 16 || pos >= it.hi) return (size_t)0;
+            return (size_t)__ldg(table + (pos >> p.page_shift)) * page_bytes + (size_t)(pos & page_mask) * row_bytes;
         };
-        int pages = page_ids(0), pages_next = 0;
+        // rows of a tile that this thread's row 0 is in front of the end by
+        const auto room_of = [&](int tile) { return chunk < (p.head >> 3) ? it.hi - (it.lo + tile * Keys) - row : 0; };
+        size_t place = places(0), place_next = 0;
         uint4 v[Loads * (F32 ? 2 : 1)];
-        const auto load = [&](int i, int k, int ids) {  // rows k * Step .. of the i-th tile of the ring
-            const int pos = it.lo + (i >> 1) * Keys + k * Step + row;
-            const int page = __shfl_sync(0xffffffffu, ids, k * Step / 16);
-            const size_t e = k_base + ((i & 1) ? v_off : 0) + (size_t)page * page_stride + (size_t)(pos & page_mask) * p.head;
-            const bool in = have && pos < it.hi;
+        const auto load = [&](int k, const char *src, size_t at, int room) {
+            const uint4 *from = reinterpret_cast<const uint4 *>(src + __shfl_sync(0xffffffffu, at, k * Step / 16) +
+                                                                (k * Step % 16) * row_bytes);
             const uint4 zero = make_uint4(0, 0, 0, 0);
+            const bool in = k * Step < room;
             if constexpr (F32) {
-                const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const float *>(p.kv) + e);
-                v[2 * k] = in ? __ldg(src) : zero;
-                v[2 * k + 1] = in ? __ldg(src + 1) : zero;
+                v[2 * k] = in ? __ldg(from) : zero;
+                v[2 * k + 1] = in ? __ldg(from + 1) : zero;
             } else {
-                v[k] = in ? __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.kv) + e)) : zero;
+                v[k] = in ? __ldg(from) : zero;
             }
         };
         if (n > 0) {
 #pragma unroll
-            for (int k = 0; k < Loads; ++k) load(0, k, pages);
+            for (int k = 0; k < Loads; ++k) load(k, k_src, place, room_of(0));
         }
         int slot = 0;
         uint32_t freed = 1;  // parity of the slot's last use; the first round finds every slot free
         for (int i = 0; i < 2 * n; ++i) {
-            if (!(i & 1)) pages_next = page_ids((i >> 1) + 1);
+            if (!(i & 1)) place_next = places((i >> 1) + 1);
             // the tile's largest magnitude, and the smallest of the chunks'
             uint32_t most = 0, least = 0xffffffffu;
+            if constexpr (F32) {
 #pragma unroll
-            for (int k = 0; k < Loads; ++k) {
-                uint32_t m;
-                if constexpr (F32) {
+                for (int k = 0; k < Loads; ++k) {
                     const uint32_t a = max(max(v[2 * k].x & 0x7fffffffu, v[2 * k].y & 0x7fffffffu),
                                            max(v[2 * k].z & 0x7fffffffu, v[2 * k].w & 0x7fffffffu));
                     const uint32_t b = max(max(v[2 * k + 1].x & 0x7fffffffu, v[2 * k + 1].y & 0x7fffffffu),
                                            max(v[2 * k + 1].z & 0x7fffffffu, v[2 * k + 1].w & 0x7fffffffu));
-                    m = max(a, b);
-                } else {
-                    const uint32_t a = __vmaxu2(v[k].x & 0x7fff7fffu, v[k].y & 0x7fff7fffu);
-                    const uint32_t b = __vmaxu2(v[k].z & 0x7fff7fffu, v[k].w & 0x7fff7fffu);
-                    const uint32_t c = __vmaxu2(a, b);
-                    m = max(c << 16, c & 0xffff0000u);
+                    const uint32_t m = max(a, b);
+                    most = max(most, m);
+                    least = min(least, m - 1);
                 }
-                most = max(most, m);
-                least = min(least, m - 1);
+            } else {  // two bf16 a register; the chunks are the four even and the four odd elements
+                uint32_t hi = 0, lo = 0xffffffffu;
+#pragma unroll
+                for (int k = 0; k < Loads; ++k) {
+                    const uint32_t m = max_u16x2(max_u16x2(v[k].x & 0x7fff7fffu, v[k].y & 0x7fff7fffu),
+                                                 max_u16x2(v[k].z & 0x7fff7fffu, v[k].w & 0x7fff7fffu));
+                    hi = max_u16x2(hi, m);
+                    lo = min_u16x2(lo, __vsub2(m, 0x00010001u));
+                }
+                most = max(hi << 16, hi & 0xffff0000u);
+                const uint32_t l0 = lo & 0xffffu, l1 = lo >> 16, l = min(l0, l1);
+                least = l == 0xffffu ? 0xffffffffu : ((l + 1) << 16) - 1;
             }
             most = __reduce_max_sync(0xffffffffu, most);
             least = __reduce_min_sync(0xffffffffu, least);
@@ -536,66 +601,63 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 if (too_wide(most, least)) s_wild = 1;
                 ((i & 1) ? s_vscale : s_kscale)[(i >> 1) & (kScaleRing - 1)] = down_scale(up);
             }
-            const uint32_t dst = slots + (uint32_t)slot * S::Slot + (uint32_t)(chunk >> 3) * S::Sub;
+            const uint32_t dst =
+                slots + (uint32_t)slot * S::Slot + (uint32_t)(chunk >> 3) * S::Sub + swizzled(row, chunk & 7);
             // a chunk's registers take the next tile's as soon as it is stored
-            const bool more = i + 1 < 2 * n;
-            const int ids = (i & 1) ? pages_next : pages;
+            // (the last tile's load again)
+            const int next = min(i + 1, 2 * n - 1);
+            const char *src = (next & 1) ? v_src : k_src;
+            const size_t at = (i & 1) && next > i ? place_next : place;
+            const int room = room_of(next >> 1);
+            const __nv_bfloat162 up2 = __float2bfloat162_rn(up);
 #pragma unroll
             for (int k = 0; k < Loads; ++k) {
                 uint4 hi, lo;
                 if constexpr (F32) {
-                    const float x[8] = {__uint_as_float(v[2 * k].x),     __uint_as_float(v[2 * k].y),
-                                        __uint_as_float(v[2 * k].z),     __uint_as_float(v[2 * k].w),
-                                        __uint_as_float(v[2 * k + 1].x), __uint_as_float(v[2 * k + 1].y),
-                                        __uint_as_float(v[2 * k + 1].z), __uint_as_float(v[2 * k + 1].w)};
-                    halves<true>(x, up, hi, lo);
+                    halves(*reinterpret_cast<const float4 *>(&v[2 * k]), *reinterpret_cast<const float4 *>(&v[2 * k + 1]),
+                           up, hi, lo);
                 } else {
-                    const float x[8] = {__uint_as_float(v[k].x << 16), __uint_as_float(v[k].x & 0xffff0000u),
-                                        __uint_as_float(v[k].y << 16), __uint_as_float(v[k].y & 0xffff0000u),
-                                        __uint_as_float(v[k].z << 16), __uint_as_float(v[k].z & 0xffff0000u),
-                                        __uint_as_float(v[k].w << 16), __uint_as_float(v[k].w & 0xffff0000u)};
-                    halves<false>(x, up, hi, lo);
+                    hi = make_uint4(to_half(v[k].x, up2), to_half(v[k].y, up2), to_half(v[k].z, up2),
+                                    to_half(v[k].w, up2));
                 }
-                const uint32_t o = dst + swizzled(k * Step + row, chunk & 7);
-                store_shared(o, hi);
-                if (F32) store_shared(o + (D / 64) * S::Sub, lo);
-                if (more) load(i + 1, k, ids);
+                // (row + k Step) & 7 = row & 7: the swizzle is the row's
+                store_shared(dst + k * Step * 128, hi);
+                if (F32) store_shared(dst + k * Step * 128 + (D / 64) * S::Sub, lo);
+                load(k, src, at, room);
             }
-            if (i & 1) pages = pages_next;
+            if (i & 1) place = place_next;
             fence_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&slot_full[slot]);
             if (++slot == S::Slots) slot = 0, freed ^= 1;
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
         if (warp == 12) {
             // ---- the MMAs: the warp waits as one, one lane issues ---------------------------------------------------------
-            // addresses in descriptors are in units of 16 bytes: offsets add
-            const uint64_t qd = sw128_desc(base), kd = sw128_desc(slots), vd = mn_desc(slots, S::Sub);
             const auto scores = [&](auto t, int slot) {  // S = (q_hi + q_lo) K^T
                 if (!elect_one()) return;
-                const uint64_t a = qd + (uint64_t)(t * S::QTile >> 4), k = kd + (uint64_t)(slot * (S::Slot >> 4));
+                const uint32_t a = here(k_desc(base + t * S::QTile)), k = here(k_desc(slots + slot * S::Slot));
 #pragma unroll
                 for (int x = 0; x < S::Parts + 1; ++x) {  // q_hi K_hi, q_lo K_hi, q_hi K_lo
                     const int qo = x == 1 ? (D / 64) * 16384 : 0, ko = x == 2 ? (D / 64) * S::Sub : 0;
 #pragma unroll
                     for (int d = 0; d < D / 16; ++d)
                         mma_ss(tmem + t * S::Region, a + ((qo + (d >> 2) * 16384 + (d & 3) * 32) >> 4),
-                               k + ((ko + (d >> 2) * S::Sub + (d & 3) * 32) >> 4), idesc<Keys, false>(), x | d);
+                               k + ((ko + (d >> 2) * S::Sub + (d & 3) * 32) >> 4), idesc<Keys, false>(x == 1, x == 2),
+                               x | d);
                 }
             };
             const auto values = [&](auto t, int slot) {  // O = (w_hi + w_lo) V
                 if (!elect_one()) return;
-                const uint64_t v = vd + (uint64_t)(slot * (S::Slot >> 4));
-                const uint32_t w = tmem + t * S::Region;
+                const uint32_t v = here(mn_desc(slots + slot * S::Slot, S::Sub)), w = here(tmem + t * S::Region);
 #pragma unroll
                 for (int x = 0; x < S::Parts + 1; ++x) {  // w_hi V_hi, w_lo V_hi, w_hi V_lo
                     const int vo = x == 2 ? (D / 64) * S::Sub : 0;
 #pragma unroll
                     for (int k = 0; k < Keys / 16; ++k)
                         mma_ts(w + Keys, w + k * 16 / W * W + k * 16 % W / 2 + (x == 1 ? W / 2 : 0), v + ((vo + k * 2048) >> 4),
-                               idesc<D, true>(), x | k);
+                               idesc<D, true>(x == 1, x == 2), x | k);
                 }
             };
             const auto commit = [&](uint64_t *bar) {

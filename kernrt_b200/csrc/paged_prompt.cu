@@ -58,7 +58,11 @@ struct Shape {
     static constexpr int QTile = 2 * (D / 64) * 128 * 128;  // both halves of 128 rows
     static constexpr size_t Smem = 2 * (size_t)QTile + (size_t)Slots * Slot + 1024;
     static constexpr int Wide = D == 64 ? 32 : 16;  // columns a softmax thread takes at a time
-    static constexpr int Region = Keys + D;  // TMEM columns of a query tile: scores / weights, sum of V
+    // TMEM columns: three buffers of scores / weights, which the two query
+    // tiles take in turn, and the sums of V of both tiles or, where they do not
+    // fit, of one at a time
+    static constexpr int Sums = 3 * Keys + 2 * D <= 512 ? 2 : 1;
+    static constexpr int SumAt = 3 * Keys;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -291,7 +295,7 @@ __device__ __forceinline__ bool loader_or(bool p) {
 }
 
 template <int T>
-struct Tile {  // a query tile, known at compile time
+struct Tile {  // a number known at compile time
     __device__ __forceinline__ constexpr operator int() const { return T; }
 };
 
@@ -302,7 +306,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     using S = Shape<D, F32>;
     constexpr int Keys = S::Keys, W = S::Wide;
     extern __shared__ unsigned char raw_smem[];
-    __shared__ uint64_t slot_full[S::Slots], slot_empty[S::Slots], s_full[2], p_full[2], q_full, done;
+    __shared__ uint64_t slot_full[S::Slots], slot_empty[S::Slots], s_full[3], p_full[2], o_full[2], o_free, q_full, done, turn[2][4];
     __shared__ uint32_t s_tmem, s_red[2][4][2];
     __shared__ float s_kscale[kScaleRing], s_vscale[kScaleRing];
     __shared__ int s_abort, s_wild;
@@ -316,10 +320,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             mbar_init(&slot_full[i], 4);
             mbar_init(&slot_empty[i], 1);
         }
+        for (int b = 0; b < 3; ++b) mbar_init(&s_full[b], 1);
         for (int t = 0; t < 2; ++t) {
-            mbar_init(&s_full[t], 1);
             mbar_init(&p_full[t], 4);
+            mbar_init(&o_full[t], 1);
         }
+        mbar_init(&o_free, 4);
+        for (int w = 0; w < 8; ++w) mbar_init(&turn[w >> 2][w & 3], 1);
         mbar_init(&q_full, 8);
         mbar_init(&done, 1);
         s_abort = 0;
@@ -345,7 +352,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const int seen = min(it.hi, sq.ctx + (it.row + last) / p.group + 1) - it.lo;
         return last < 128 * t || seen <= 0 ? 0 : (seen + Keys - 1) / Keys;
     };
+    // (rows ascend, so n0 <= n1 unless there is no second tile)
     const int n0 = tiles_of(0), n1 = tiles_of(1), n = max(n0, n1);
+    // The order of the work on (key tile i, query tile t): the s-th takes score
+    // buffer s % 3.
+    //   s = 2 i + t while both tiles have keys, then n0 + i; n1 = 0: s = i
 
     const auto wait = [&](uint64_t *bar, uint32_t parity) {
         if (mbar_try_wait(bar, parity)) return true;
@@ -414,37 +425,55 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         for (int d = 0; d < D / 2; ++d) acc[d] = both(0.0f);
         float m = -INFINITY, l = 0.0f;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t s_at = tmem + lanes + (uint32_t)(t * S::Region), o_at = s_at + Keys;
-        const auto flush = [&](int tile) {  // the tile's sum of V into the registers
+        const uint32_t o_at = tmem + lanes + (uint32_t)(S::SumAt + (S::Sums == 2 ? t * D : 0));
+        // the sum of V over a key tile, once it is there, into the registers
+        const auto flush = [&](int tile) {
+            if (!__all_sync(0xffffffffu, wait(&o_full[t], (uint32_t)tile & 1u))) return false;
+            tc_fence_after();
             const float vs = s_vscale[tile & (kScaleRing - 1)];
             tmem_each<D, W>(o_at, [&](int c, uint32_t(&v)[W]) {
 #pragma unroll
                 for (int i = 0; i < W / 2; ++i)
                     acc[c / 2 + i] = fma2(pair(v[2 * i], v[2 * i + 1]), both(vs), acc[c / 2 + i]);
             });
+            if constexpr (S::Sums == 1) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&o_free);
+            }
+            return true;
         };
         bool ok = true;
         const int mine = t ? n1 : n0;
-        for (int tile = 0; tile < mine; ++tile) {
-            ok = __all_sync(0xffffffffu, wait(&s_full[t], (uint32_t)tile & 1u));
+        int buf = t && n0 > 0;  // s = t, or 0 where tile 1 is alone
+        uint32_t round = 0;
+        for (int tile = 0; ok && tile < mine; ++tile) {
+            ok = __all_sync(0xffffffffu, wait(&s_full[buf], round));
             if (!ok) break;
             tc_fence_after();
+            const uint32_t s_at = tmem + lanes + (uint32_t)(buf * Keys);
+            buf += n1 > 0 && tile + 1 < (t ? n0 : mine) ? 2 : 1;
+            if (buf >= 3) buf -= 3, round ^= 1;
             const int rem = limit - (it.lo + tile * Keys);  // the tile's keys this row sees
             const bool masked = __any_sync(0xffffffffu, rem < Keys);
             const float ks = sc * s_kscale[tile & (kScaleRing - 1)];
             float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            tmem_each<Keys, W>(s_at, [&](int c, uint32_t(&v)[W]) {
+            // (rolled loops: the roles' code competes for the instruction caches)
+#pragma unroll 1
+            for (int c = 0; c < Keys; c += 32) {
+                uint32_t v[32];
+                Tmem<32>::load(s_at + (uint32_t)c, v);
+                Tmem<32>::wait(v);
                 if (masked) {
 #pragma unroll
-                    for (int i = 0; i < W; ++i)
+                    for (int i = 0; i < 32; ++i)
                         if (c + i >= rem) v[i] = 0xff800000u;  // -inf
                 }
 #pragma unroll
-                for (int i = 0; i < W; i += 2)
-                    part[i / 2 & 3] = max3(part[i / 2 & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-            });
+                for (int i = 0; i < 32; ++i) part[i & 3] = fmaxf(part[i & 3], __uint_as_float(v[i]));
+            }
             const float mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-            if (tile) flush(tile - 1);
+            if (S::Sums == 2 && tile && !(ok = flush(tile - 1))) break;
             const float mn = fmaxf(m, mx * ks);
             if (tile && __any_sync(0xffffffffu, mn > m)) {
                 const float keep = mn == -INFINITY ? 0.0f : ex2(m - mn);
@@ -453,36 +482,50 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 for (int d = 0; d < D / 2; ++d) acc[d] = mul2(acc[d], both(keep));
             }
             m = mn;
+            // The exponentials of warp w of both query tiles share one pair of
+            // units (16 a cycle and SM); taken in turns, each runs under the other's
+            // remaining work, where both at once would leave the units idle after.
+            const bool paired = n1 > 0 && tile < n0;
+            if (paired && t + tile > 0) {
+                ok = __all_sync(0xffffffffu, wait(&turn[t][warp & 3], (uint32_t)(tile - 1 + t) & 1u));
+                if (!ok) break;
+            }
             // weights times 2^14: the halves of small ones stay normal numbers
             const float bias = 14.0f - (m == -INFINITY ? 0.0f : m);
             F2 sum[2] = {both(0.0f), both(0.0f)};
-            tmem_each<Keys, W>(s_at, [&](int c, uint32_t(&v)[W]) {
-                // in place: W / 2 columns of the halves hi, W / 2 of -lo
-                uint32_t h[W];
+            const auto weights = [&](auto some_masked) {
+#pragma unroll 1
+                for (int c = 0; c < Keys; c += W) {
+                    uint32_t v[W], h[W];
+                    Tmem<W>::load(s_at + (uint32_t)c, v);
+                    Tmem<W>::wait(v);
+                    // in place: W / 2 columns of the halves hi, W / 2 of -lo
 #pragma unroll
-                for (int i = 0; i < W / 2; ++i) {
-                    const F2 x = fma2(pair(v[2 * i], v[2 * i + 1]), both(ks), both(bias));
-                    F2 w{ex2(x.x), ex2(x.y)};
-                    if (masked) {
-                        if (c + 2 * i >= rem) w.x = 0.0f;
-                        if (c + 2 * i + 1 >= rem) w.y = 0.0f;
+                    for (int i = 0; i < W / 2; ++i) {
+                        const F2 x = fma2(pair(v[2 * i], v[2 * i + 1]), both(ks), both(bias));
+                        F2 w{ex2(x.x), ex2(x.y)};
+                        if (some_masked) {
+                            if (c + 2 * i >= rem) w.x = 0.0f;
+                            if (c + 2 * i + 1 >= rem) w.y = 0.0f;
+                        }
+                        sum[i & 1] = add2(sum[i & 1], w);
+                        split_half(w, h[i], h[W / 2 + i]);
                     }
-                    sum[i & 1] = add2(sum[i & 1], w);
-                    split_half(w, h[i], h[W / 2 + i]);
+                    Tmem<W>::store(s_at + (uint32_t)c, h);
                 }
-                Tmem<W>::store(s_at + (uint32_t)c, h);
-            });
+            };
+            if (masked) weights(Tile<1>{});
+            else weights(Tile<0>{});
+            __syncwarp();
+            if (paired && lane == 0) mbar_arrive(&turn[t ^ 1][warp & 3]);
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[t]);
+            if (S::Sums == 1) ok = flush(tile);
         }
-        if (ok && mine) {
-            ok = __all_sync(0xffffffffu, wait(&s_full[t], (uint32_t)mine & 1u));
-            tc_fence_after();
-            if (ok) flush(mine - 1);
-        }
+        if (S::Sums == 2 && ok && mine) ok = flush(mine - 1);
         if (ok) {
             bool fine = isfinite(l) && !*(volatile int *)&s_wild;
 #pragma unroll
@@ -514,7 +557,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
         }
     } else if (warp < 12) {
-        // ---- the loader: tiles K0 V0 K1 V1 .. ---------------------------------
+        // ---- the loader: tiles K0 K1 V0 K2 V1 .. V(n-1) ---------------------------------
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         constexpr int PerRow = D / 8, Step = 128 / PerRow;  // eight-element chunks of a row, rows of a step
         constexpr int Loads = Keys / Step;
@@ -526,7 +569,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const char *k_src = static_cast<const char *>(p.kv) + (page_elem(p, layer, 0, 0, j) + 8 * chunk) * Size +
                             (size_t)row * row_bytes;
         const char *v_src = k_src + (page_elem(p, layer, 1, 0, j) - page_elem(p, layer, 0, 0, j)) * Size;
-        // lane i: where positions 16 i .. of a tile lie; kept one tile ahead
+        // lane i: where positions 16 i .. of a tile lie
         const auto places = [&](int tile) {
             const int pos = it.lo + tile * Keys + 16 * lane;
             if (lane >= Keys / 16 || pos >= it.hi) return (size_t)0;
@@ -534,7 +577,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         };
         // rows of a tile that this thread's row 0 is in front of the end by
         const auto room_of = [&](int tile) { return chunk < (p.head >> 3) ? it.hi - (it.lo + tile * Keys) - row : 0; };
-        size_t place = places(0), place_next = 0;
+        const auto is_v = [&](int i) { return i == 2 * n - 1 || (i > 0 && !(i & 1)); };
+        const auto tile_of = [&](int i) { return i == 2 * n - 1 ? n - 1 : is_v(i) ? i / 2 - 1 : (i + 1) / 2; };
+        size_t place = places(tile_of(1));  // of the tile after the one in registers
         uint4 v[Loads * (F32 ? 2 : 1)];
         const auto load = [&](int k, const char *src, size_t at, int room) {
             const uint4 *from = reinterpret_cast<const uint4 *>(src + __shfl_sync(0xffffffffu, at, k * Step / 16) +
@@ -549,13 +594,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
         };
         if (n > 0) {
+            const size_t first = places(0);
 #pragma unroll
-            for (int k = 0; k < Loads; ++k) load(k, k_src, place, room_of(0));
+            for (int k = 0; k < Loads; ++k) load(k, k_src, first, room_of(0));
         }
         int slot = 0;
         uint32_t freed = 1;  // parity of the slot's last use; the first round finds every slot free
         for (int i = 0; i < 2 * n; ++i) {
-            if (!(i & 1)) place_next = places((i >> 1) + 1);
+            const int next = min(i + 1, 2 * n - 1);
+            const size_t place_next = places(tile_of(min(i + 2, 2 * n - 1)));
             // the tile's largest magnitude, and the smallest of the chunks'
             uint32_t most = 0, least = 0xffffffffu;
             if constexpr (F32) {
@@ -599,16 +646,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             const float up = up_scale(most);
             if (tid == 0) {
                 if (too_wide(most, least)) s_wild = 1;
-                ((i & 1) ? s_vscale : s_kscale)[(i >> 1) & (kScaleRing - 1)] = down_scale(up);
+                (is_v(i) ? s_vscale : s_kscale)[tile_of(i) & (kScaleRing - 1)] = down_scale(up);
             }
             const uint32_t dst =
                 slots + (uint32_t)slot * S::Slot + (uint32_t)(chunk >> 3) * S::Sub + swizzled(row, chunk & 7);
             // a chunk's registers take the next tile's as soon as it is stored
             // (the last tile's load again)
-            const int next = min(i + 1, 2 * n - 1);
-            const char *src = (next & 1) ? v_src : k_src;
-            const size_t at = (i & 1) && next > i ? place_next : place;
-            const int room = room_of(next >> 1);
+            const char *src = is_v(next) ? v_src : k_src;
+            const int room = room_of(tile_of(next));
             const __nv_bfloat162 up2 = __float2bfloat162_rn(up);
 #pragma unroll
             for (int k = 0; k < Loads; ++k) {
@@ -623,9 +668,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 // (row + k Step) & 7 = row & 7: the swizzle is the row's
                 store_shared(dst + k * Step * 128, hi);
                 if (F32) store_shared(dst + k * Step * 128 + (D / 64) * S::Sub, lo);
-                load(k, src, at, room);
+                load(k, src, place, room);
             }
-            if (i & 1) place = place_next;
+            place = place_next;
             fence_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&slot_full[slot]);
@@ -635,28 +680,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
         if (warp == 12) {
             // ---- the MMAs: the warp waits as one, one lane issues ---------------------------------------------------------
-            const auto scores = [&](auto t, int slot) {  // S = (q_hi + q_lo) K^T
+            const auto scores = [&](auto t, int slot, int buf) {  // S = (q_hi + q_lo) K^T
                 if (!elect_one()) return;
                 const uint32_t a = here(k_desc(base + t * S::QTile)), k = here(k_desc(slots + slot * S::Slot));
+                const uint32_t d_at = here(tmem + buf * Keys);
 #pragma unroll
                 for (int x = 0; x < S::Parts + 1; ++x) {  // q_hi K_hi, q_lo K_hi, q_hi K_lo
                     const int qo = x == 1 ? (D / 64) * 16384 : 0, ko = x == 2 ? (D / 64) * S::Sub : 0;
 #pragma unroll
                     for (int d = 0; d < D / 16; ++d)
-                        mma_ss(tmem + t * S::Region, a + ((qo + (d >> 2) * 16384 + (d & 3) * 32) >> 4),
+                        mma_ss(d_at, a + ((qo + (d >> 2) * 16384 + (d & 3) * 32) >> 4),
                                k + ((ko + (d >> 2) * S::Sub + (d & 3) * 32) >> 4), idesc<Keys, false>(x == 1, x == 2),
                                x | d);
                 }
             };
-            const auto values = [&](auto t, int slot) {  // O = (w_hi + w_lo) V
+            const auto values = [&](auto t, int slot, int buf) {  // O = (w_hi + w_lo) V
                 if (!elect_one()) return;
-                const uint32_t v = here(mn_desc(slots + slot * S::Slot, S::Sub)), w = here(tmem + t * S::Region);
+                const uint32_t v = here(mn_desc(slots + slot * S::Slot, S::Sub)), w = here(tmem + buf * Keys);
+                const uint32_t d_at = here(tmem + S::SumAt + (S::Sums == 2 ? t * D : 0));
 #pragma unroll
                 for (int x = 0; x < S::Parts + 1; ++x) {  // w_hi V_hi, w_lo V_hi, w_hi V_lo
                     const int vo = x == 2 ? (D / 64) * S::Sub : 0;
 #pragma unroll
                     for (int k = 0; k < Keys / 16; ++k)
-                        mma_ts(w + Keys, w + k * 16 / W * W + k * 16 % W / 2 + (x == 1 ? W / 2 : 0), v + ((vo + k * 2048) >> 4),
+                        mma_ts(d_at, w + k * 16 / W * W + k * 16 % W / 2 + (x == 1 ? W / 2 : 0), v + ((vo + k * 2048) >> 4),
                                idesc<D, true>(x == 1, x == 2), x | k);
                 }
             };
@@ -664,49 +711,64 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 if (elect_one()) mma_commit(bar);
             };
             const auto wait_all = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
-            struct Place {  // of the K or V tiles in the ring
-                int slot;
+            struct Ring {  // a place in a ring of N, and the parity of its round
+                int at;
                 uint32_t parity;
-                __device__ __forceinline__ void next() {
-                    slot += 2;
-                    if (slot >= S::Slots) slot -= S::Slots, parity ^= 1;
+                __device__ __forceinline__ void advance(int by, int n) {
+                    at += by;
+                    if (at >= n) at -= n, parity ^= 1;
                 }
             };
-            Place kp{0, 0}, vp{1, 0};
-            bool ok = wait_all(&q_full, 0) && (n == 0 || wait_all(&slot_full[0], 0));
-            if (ok && n > 0) {
+            // Tiles of K come at 0, 1, 3, 5 .. of the slots' order, of V at 2, 4
+            // .. 2 n - 2 and 2 n - 1.
+            Ring kp{0, 0}, vp{n > 1 ? 2 : 1, 0};
+            int sb = 0, pb = 0;  // score buffers of the next scores and values
+            uint32_t freed = 1;  // parity for o_free: the first sum finds its place free
+            bool ok = wait_all(&q_full, 0);
+            const auto next_scores = [&](auto t, int tile, bool last_use) {
+                if (!wait_all(&slot_full[kp.at], kp.parity)) return false;
                 tc_fence_after();
-                if (n0 > 0) {
-                    scores(Tile<0>{}, 0);
-                    commit(&s_full[0]);
+                scores(t, kp.at, sb);
+                commit(&s_full[sb]);
+                sb = sb == 2 ? 0 : sb + 1;
+                if (last_use) {  // by the last query tile that reads it
+                    commit(&slot_empty[kp.at]);
+                    kp.advance(tile ? 2 : 1, S::Slots);
                 }
-                if (n1 > 0) {
-                    scores(Tile<1>{}, 0);
-                    commit(&s_full[1]);
+                return true;
+            };
+            const auto next_values = [&](auto t, int tile, bool last_use) {
+                if (!wait_all(&slot_full[vp.at], vp.parity) || !wait_all(&p_full[t], (uint32_t)tile & 1u)) return false;
+                if (S::Sums == 1) {
+                    if (!wait_all(&o_free, freed)) return false;
+                    freed ^= 1;
                 }
-                commit(&slot_empty[0]);
-                kp.next();
-            }
+                tc_fence_after();
+                values(t, vp.at, pb);
+                commit(&o_full[t]);
+                pb = pb == 2 ? 0 : pb + 1;
+                if (last_use) {
+                    commit(&slot_empty[vp.at]);
+                    vp.advance(tile + 2 < n ? 2 : 1, S::Slots);
+                }
+                return true;
+            };
+            // The scores run three pieces of work ahead of the values.
+            Tile<0> first;
+            Tile<1> second;
+            int st = n0 > 0 ? 0 : 1, si = 0;  // the next scores' query and key tile
+            const auto advance_scores = [&]() {
+                if (si >= n) return true;
+                const bool both_have = n1 > 0 && si < n0;
+                const bool fine = st ? next_scores(second, si, true) : next_scores(first, si, !both_have);
+                if (st == 0 && both_have) st = 1;
+                else ++si, st = n0 > si ? 0 : 1;
+                return fine;
+            };
+            for (int k = 0; ok && k < 3; ++k) ok = advance_scores();
             for (int tile = 0; ok && tile < n; ++tile) {
-                const auto turn = [&](auto t, int mine) {
-                    if (tile >= mine) return true;
-                    if (!wait_all(&slot_full[vp.slot], vp.parity) || !wait_all(&p_full[t], (uint32_t)tile & 1u)) return false;
-                    tc_fence_after();
-                    values(t, vp.slot);
-                    if (tile + 1 < mine) {
-                        if (!wait_all(&slot_full[kp.slot], kp.parity)) return false;
-                        tc_fence_after();
-                        scores(t, kp.slot);
-                    }
-                    commit(&s_full[t]);
-                    return true;
-                };
-                ok = turn(Tile<0>{}, n0) && turn(Tile<1>{}, n1);
-                if (!ok) break;
-                commit(&slot_empty[vp.slot]);
-                if (tile + 1 < n) commit(&slot_empty[kp.slot]);
-                vp.next();
-                kp.next();
+                if (tile < n0) ok = next_values(first, tile, n1 == 0) && advance_scores();
+                if (ok && tile < n1) ok = next_values(second, tile, true) && advance_scores();
             }
             commit(&done);  // every MMA issued, finished loop or not
         }

@@ -133,9 +133,11 @@ int kernrt_cuda_read_bytes(kernrt_cuda_ctx *ctx, kernrt_buf src, size_t src_byte
                            size_t bytes);
 /* Device address of a buffer (valid until destroy), for zero-copy interop. */
 int kernrt_cuda_device_ptr(kernrt_cuda_ctx *ctx, kernrt_buf buf, void **ptr);
-/* Gives a buffer's memory back once the work already enqueued is done (the
- * trait frees nothing before the backend goes; a serving process outlives its
- * requests).  The handle is invalid from then on and is not used again. */
+/* Gives a buffer's memory back (the trait frees nothing before the backend
+ * goes; a serving process outlives its requests).  The handle is invalid from
+ * then on and is not used again.  The context keeps freed memory, at most 8 GB
+ * of it, for its next allocations, whose work is ordered behind the work already
+ * enqueued; work of the caller's own on other streams has to be done. */
 int kernrt_cuda_free(kernrt_cuda_ctx *ctx, kernrt_buf buf);
 /* Wait for all deferred work. */
 int kernrt_cuda_synchronize(kernrt_cuda_ctx *ctx);
@@ -410,7 +412,7 @@ typedef uint64_t kernrt_pages;
 int kernrt_cuda_pages_create(kernrt_cuda_ctx *ctx, int kind, size_t n_layers, size_t n_heads, size_t n_kv_heads,
                              size_t head_size, size_t page_size, size_t n_pages, size_t max_seqs, size_t max_len,
                              kernrt_pages *out);
-/* Frees it once the work already enqueued is done. */
+/* Gives its memory back, as kernrt_cuda_free does a buffer's. */
 int kernrt_cuda_pages_destroy(kernrt_cuda_ctx *ctx, kernrt_pages pages);
 
 /* The pages' device address (valid until pages_destroy; zero-copy interop, to

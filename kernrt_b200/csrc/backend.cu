@@ -94,6 +94,7 @@ public:
         cudaFree(vc_);
         cudaFree(att_scratch_);
         for (auto &c : caches_) free_cache(c);
+        drop_spare(0);
         cudaFree(d_err_);
         cudaFree(d_ticket_);
         cudaFree(split_);
@@ -360,7 +361,7 @@ public:
         // Fault injection for tests: KERNRT_CUDA_FAIL_ALLOC=n makes this
         // context's n-th buffer allocation fail as an exhausted device would.
         if (++allocs_ == fail_alloc_at_) check(cudaErrorMemoryAllocation, "cudaMalloc");
-        check(cudaMalloc(&b.ptr, std::max<size_t>(bytes, 16)), "cudaMalloc");
+        b.ptr = static_cast<char *>(take_block(bytes, "cudaMalloc"));
         check(cudaMemsetAsync(b.ptr, 0, std::max<size_t>(bytes, 16), stream_), "cudaMemset");
         bufs_.push_back(b);
         return (kernrt_buf)bufs_.size();  // handle = index + 1; 0 means "none"
@@ -402,14 +403,57 @@ public:
 
     void *device_ptr(kernrt_buf h) { return buf(h).ptr; }
 
-    // Gives a buffer's memory back once the work already queued on it is done;
-    // its handle is not used again.
+    // Gives a buffer's memory back; its handle is not used again.
     void free_buf(kernrt_buf h) {
         Buffer &b = buf(h);
         flush();
-        check(cudaStreamSynchronize(stream_), "synchronize");
-        cudaFree(b.ptr);
+        give_block(b.ptr, b.bytes);
         b = Buffer{};
+    }
+
+    // Device memory by size, for buffers and caches that come and go: a freed
+    // block is kept for the next allocation of its size, at most kSpareMax bytes in
+    // all (the longest kept go first).  No call waits: whoever takes a block
+    // works on stream_, behind the work that still uses it.  cudaMalloc and
+    // cudaFree were measured at 0.1 to 100 ms a call on a shared machine.
+    static constexpr size_t kSpareMax = (size_t)8 << 30;
+    static size_t block_size(size_t bytes) {
+        const size_t unit = bytes < ((size_t)1 << 20) ? 512 : (size_t)2 << 20;
+        return (std::max<size_t>(bytes, 16) + unit - 1) / unit * unit;
+    }
+    void *take_block(size_t bytes, const char *what) {
+        const size_t size = block_size(bytes);
+        for (size_t i = 0; i < spare_.size(); ++i)
+            if (spare_[i].bytes == size) {
+                void *p = spare_[i].ptr;
+                spare_.erase(spare_.begin() + (long)i);
+                spare_bytes_ -= size;
+                return p;
+            }
+        void *p = nullptr;
+        cudaError_t e = cudaMalloc(&p, size);
+        if (e == cudaErrorMemoryAllocation && !spare_.empty()) {
+            cudaGetLastError();
+            drop_spare(0);
+            e = cudaMalloc(&p, size);
+        }
+        if (e != cudaSuccess) cudaGetLastError();
+        check(e, what);
+        return p;
+    }
+    void give_block(void *p, size_t bytes) {
+        if (!p) return;
+        spare_.push_back({static_cast<char *>(p), block_size(bytes)});
+        spare_bytes_ += block_size(bytes);
+        drop_spare(kSpareMax);
+    }
+    void drop_spare(size_t keep) {  // cudaFree waits for queued work that may use the block
+        size_t n = 0;
+        while (spare_bytes_ > keep) {
+            spare_bytes_ -= spare_[n].bytes;
+            cudaFree(spare_[n++].ptr);
+        }
+        spare_.erase(spare_.begin(), spare_.begin() + (long)n);
     }
 
     // Completes deferred work and surfaces device-reported input errors.
@@ -1345,33 +1389,44 @@ public:
     }
 
     // ---- paged key/value caches (pages.h: the bookkeeping; paged.cu: the device) ----
+    struct Grown {
+        void *ptr = nullptr;
+        size_t bytes = 0;
+    };
     struct PagedCache {
         std::unique_ptr<PageMap> map;  // null once destroyed
         PagesView view{};
+        size_t kv_bytes = 0, table_bytes = 0;
         int32_t *table = nullptr;
-        StepSeq *seqs = nullptr;  // the current step's descriptors [max_seqs]
-        bool stepped = false;     // a step is planned and its tables are current
-        size_t n = 0, rows = 0;   // its sequences (those with rows) and rows
-        // the attention's pieces of the step and their scratch, grown as needed
-        // (decode: pieces of few rows, prompt: of many)
-        AttnItem *items = nullptr;
-        size_t items_cap = 0, n_decode = 0, n_prompt = 0;
+        StepSeq *seqs = nullptr;    // the current step's descriptors [max_seqs]
+        std::vector<StepSeq> step;  // the same on the host: its sequences with rows
+        bool stepped = false;       // a step is planned and its tables are current
+        size_t rows = 0;            // its rows
+        // the step's attention in pieces, planned at its first attention call
+        // (decode: pieces of few rows, prompt: of many), and their scratch
+        bool planned = false;
+        size_t n_decode = 0, n_prompt = 0;
         bool split_prompt = false;
-        AttnScratch decode{}, prompt{};
-        size_t decode_cap = 0, joins_cap = 0, prompt_cap = 0;  // in pieces, joins, pieces
+        Grown items, decode_o, decode_ml, decode_count, prompt_o, prompt_ml;
     };
 
-    static void free_cache(PagedCache &c) {
-        cudaFree(c.view.kv);
-        cudaFree(c.table);
-        cudaFree(c.seqs);
-        cudaFree(c.items);
-        for (AttnScratch *w : {&c.decode, &c.prompt}) {
-            cudaFree(w->o);
-            cudaFree(w->ml);
-            cudaFree(w->count);
-        }
+    void free_cache(PagedCache &c) {
+        give_block(c.view.kv, c.kv_bytes);
+        give_block(c.table, c.table_bytes);
+        if (c.map) give_block(c.seqs, c.map->max_seqs() * sizeof(StepSeq));
+        for (Grown *g : {&c.items, &c.decode_o, &c.decode_ml, &c.decode_count, &c.prompt_o, &c.prompt_ml})
+            give_block(g->ptr, g->bytes);
         c = PagedCache{};
+    }
+
+    // A block that grows to what a step needs.
+    bool grow(Grown &g, size_t bytes) {
+        if (bytes <= g.bytes) return false;
+        give_block(g.ptr, g.bytes);
+        g = Grown{};
+        g.ptr = take_block(bytes, "cudaMalloc(attention scratch)");
+        g.bytes = bytes;
+        return true;
     }
 
     uint64_t pages_create(int kind, size_t n_layers, size_t n_heads, size_t n_kv_heads, size_t head_size,
@@ -1396,11 +1451,13 @@ public:
         c.map = std::make_unique<PageMap>(n_pages, page_size, max_seqs, max_len);
         const size_t bytes = n_layers * 2 * n_pages * n_kv_heads * page_size * head_size * (kind == KERNRT_F32 ? 4 : 2);
         try {
-            check(cudaMalloc(&c.view.kv, bytes), "cudaMalloc(pages)");
-            check(cudaMalloc(&c.table, max_seqs * max_pages * sizeof(int32_t)), "cudaMalloc(page tables)");
-            check(cudaMalloc(&c.seqs, max_seqs * sizeof(StepSeq)), "cudaMalloc(step)");
+            c.kv_bytes = bytes;
+            c.table_bytes = max_seqs * max_pages * sizeof(int32_t);
+            c.view.kv = take_block(bytes, "cudaMalloc(pages)");
+            c.table = static_cast<int32_t *>(take_block(c.table_bytes, "cudaMalloc(page tables)"));
+            c.seqs = static_cast<StepSeq *>(take_block(max_seqs * sizeof(StepSeq), "cudaMalloc(step)"));
             check(cudaMemsetAsync(c.view.kv, 0, bytes, stream_), "cudaMemset");
-            check(cudaMemsetAsync(c.table, 0, max_seqs * max_pages * sizeof(int32_t), stream_), "cudaMemset");
+            check(cudaMemsetAsync(c.table, 0, c.table_bytes, stream_), "cudaMemset");
         } catch (...) {
             free_cache(c);
             throw;
@@ -1429,7 +1486,6 @@ public:
     void pages_destroy(uint64_t h) {
         PagedCache &c = cache(h);
         flush();
-        check(cudaStreamSynchronize(stream_), "synchronize");
         free_cache(c);
     }
 
@@ -1578,36 +1634,25 @@ public:
         a.prompt = std::move(cut);
     }
 
-    // Room for the step's pieces (memory grown under queued work is freed
-    // after it; counters start, and stay between launches, at 0).
-    void grow_plan(PagedCache &c, const AttnPlan &a) {
-        const size_t hk = (size_t)c.view.kv_heads, items = a.decode.size() + a.prompt.size();
-        const auto regrow = [&](auto *&ptr, size_t bytes, const char *what) {
-            cudaFree(ptr);
-            ptr = nullptr;
-            check(cudaMalloc(&ptr, bytes), what);
-        };
-        const auto scratch = [&](AttnScratch &w, size_t &cap, size_t parts, size_t rows) {
-            if (parts <= cap) return;
-            cap = 0;
-            regrow(w.o, parts * hk * rows * c.view.head * sizeof(float), "cudaMalloc(attention scratch)");
-            regrow(w.ml, parts * hk * rows * sizeof(float2), "cudaMalloc(attention scratch)");
-            cap = parts;
-        };
-        if (items > c.items_cap) {
-            const size_t cap = std::max<size_t>(64, 2 * items);
-            c.items_cap = 0;
-            regrow(c.items, cap * sizeof(AttnItem), "cudaMalloc(attention items)");
-            c.items_cap = cap;
-        }
-        scratch(c.decode, c.decode_cap, a.decode_parts, kDecodeRows);
-        scratch(c.prompt, c.prompt_cap, a.prompt_parts, kPromptRows);
-        if (a.joins > c.joins_cap) {
-            c.joins_cap = 0;
-            regrow(c.decode.count, a.joins * hk * sizeof(unsigned), "cudaMalloc(attention scratch)");
-            check(cudaMemsetAsync(c.decode.count, 0, a.joins * hk * sizeof(unsigned), stream_), "cudaMemset");
-            c.joins_cap = a.joins;
-        }
+    // Plans the step's attention and lays the pieces down for its layers
+    // (counters start, and stay between launches, at 0).
+    void plan_step(PagedCache &c) {
+        const AttnPlan a = plan_attention(c.view, c.step);
+        const size_t hk = (size_t)c.view.kv_heads, row = (size_t)c.view.head * sizeof(float);
+        std::vector<AttnItem> items = a.decode;
+        items.insert(items.end(), a.prompt.begin(), a.prompt.end());
+        grow(c.items, std::max<size_t>(64, items.size()) * sizeof(AttnItem));
+        grow(c.decode_o, a.decode_parts * hk * kDecodeRows * row);
+        grow(c.decode_ml, a.decode_parts * hk * kDecodeRows * sizeof(float2));
+        grow(c.prompt_o, a.prompt_parts * hk * kPromptRows * row);
+        grow(c.prompt_ml, a.prompt_parts * hk * kPromptRows * sizeof(float2));
+        if (grow(c.decode_count, a.joins * hk * sizeof(unsigned)))
+            check(cudaMemsetAsync(c.decode_count.ptr, 0, c.decode_count.bytes, stream_), "cudaMemset");
+        stage(items.data(), items.size() * sizeof(AttnItem), false, c.items.ptr);
+        c.n_decode = a.decode.size();
+        c.n_prompt = a.prompt.size();
+        c.split_prompt = a.prompt_parts > 0;
+        c.planned = true;
     }
 
     // The next step of the sequences: each grows by its rows, its table goes
@@ -1647,32 +1692,19 @@ public:
             desc.push_back(d);
             row0 += (size_t)rows[i];
         }
-        c.n = desc.size();
         c.rows = row0;
-        if (c.n) {
-            const AttnPlan plan = plan_attention(c.view, desc);
-            grow_plan(c, plan);
-            c.n_decode = plan.decode.size();
-            c.n_prompt = plan.prompt.size();
-            c.split_prompt = plan.prompt_parts > 0;
-            const size_t n_items = c.n_decode + c.n_prompt;
-            std::vector<char> block(desc.size() * sizeof(StepSeq) + n_items * sizeof(AttnItem) +
-                                    delta.size() * sizeof(int32_t));
-            char *to = block.data();
-            const auto put = [&](const void *src, size_t bytes) {
-                if (bytes) std::memcpy(to, src, bytes);
-                to += bytes;
-            };
-            put(desc.data(), desc.size() * sizeof(StepSeq));
-            put(plan.decode.data(), c.n_decode * sizeof(AttnItem));
-            put(plan.prompt.data(), c.n_prompt * sizeof(AttnItem));
-            put(delta.data(), delta.size() * sizeof(int32_t));
+        c.planned = false;
+        if (!desc.empty()) {
+            const size_t a = desc.size() * sizeof(StepSeq), b = delta.size() * sizeof(int32_t);
+            std::vector<char> block(a + b);
+            std::memcpy(block.data(), desc.data(), a);
+            if (b) std::memcpy(block.data() + a, delta.data(), b);
             const auto *d = static_cast<const StepSeq *>(stage(block.data(), block.size()));
-            launch_or_fail(launch_pages_step(d, (int)c.n, (int)n_items, c.seqs, c.items, c.table, c.view.max_pages,
-                                             stream_),
+            launch_or_fail(launch_pages_step(d, (int)desc.size(), c.seqs, c.table, c.view.max_pages, stream_),
                            "pages_step");
-            for (const StepSeq &d2 : desc) c.map->at((size_t)d2.slot).dirty = c.map->at((size_t)d2.slot).pages.size();
+            for (const StepSeq &q : desc) c.map->at((size_t)q.slot).dirty = c.map->at((size_t)q.slot).pages.size();
         }
+        c.step = std::move(desc);
         c.stepped = true;
     }
 
@@ -1690,7 +1722,7 @@ public:
         span(kb, 0, c.rows * width, "pages_write k");
         span(vb, 0, c.rows * width, "pages_write v");
         flush();
-        launch_or_fail(launch_pages_write(c.view, (int)layer, c.seqs, (int)c.n, (int)c.rows, f(kb), f(vb), stream_),
+        launch_or_fail(launch_pages_write(c.view, (int)layer, c.seqs, (int)c.step.size(), (int)c.rows, f(kb), f(vb), stream_),
                        "pages_write");
     }
 
@@ -1703,11 +1735,16 @@ public:
         span(ob, 0, c.rows * width, "pages_attention out");
         flush();
         if (c.rows == 0) return;
-        launch_or_fail(launch_pages_decode(c.view, (int)layer, c.seqs, c.items, (int)c.n_decode, c.decode, f(qb),
-                                           f(ob), stream_),
+        if (!c.planned) plan_step(c);
+        const AttnItem *items = static_cast<const AttnItem *>(c.items.ptr);
+        const AttnScratch decode{static_cast<float *>(c.decode_o.ptr), static_cast<float2 *>(c.decode_ml.ptr),
+                                 static_cast<unsigned *>(c.decode_count.ptr)};
+        const AttnScratch prompt{static_cast<float *>(c.prompt_o.ptr), static_cast<float2 *>(c.prompt_ml.ptr), nullptr};
+        launch_or_fail(launch_pages_decode(c.view, (int)layer, c.seqs, items, (int)c.n_decode, decode, f(qb), f(ob),
+                                           stream_),
                        "pages_attention");
-        launch_or_fail(launch_pages_prompt(c.view, (int)layer, c.seqs, c.items + c.n_decode, (int)c.n_prompt,
-                                           c.split_prompt, c.prompt, f(qb), f(ob), d_err_, stream_),
+        launch_or_fail(launch_pages_prompt(c.view, (int)layer, c.seqs, items + c.n_decode, (int)c.n_prompt,
+                                           c.split_prompt, prompt, f(qb), f(ob), d_err_, stream_),
                        "pages_attention (tensor cores)");
     }
 
@@ -2009,10 +2046,10 @@ private:
     // region is never rewritten while a copy from it or a kernel reading it
     // may be pending, and the stream is never drained.  A slice larger than a
     // segment grows the ring; the old one is retired, not freed, until the
-    // next barrier.
+    // next barrier.  With `to` the slice is uploaded there instead, to stay.
     static constexpr int kStageSegs = 8;
     static constexpr size_t kStageMapped = 64;  // slices read in place through the mapping
-    void *stage(const void *src, size_t bytes, bool in_place = false) {
+    void *stage(const void *src, size_t bytes, bool in_place = false, void *to = nullptr) {
         const size_t need = (bytes + 255) & ~(size_t)255;
         size_t seg = stage_cap_ / kStageSegs;
         if (need > seg) {
@@ -2039,8 +2076,9 @@ private:
         char *d = stage_dev_ + at;
         std::memcpy(h, src, bytes);
         if (in_place && bytes <= kStageMapped && stage_map_) return stage_map_ + at;
-        check(cudaMemcpyAsync(d, h, bytes, cudaMemcpyHostToDevice, stream_), "stage");
-        return d;
+        void *dst = to ? to : d;
+        check(cudaMemcpyAsync(dst, h, bytes, cudaMemcpyHostToDevice, stream_), "stage");
+        return dst;
     }
 
     void grow_staging(size_t cap) {
@@ -2137,6 +2175,8 @@ private:
     std::vector<Pending> pending_;
     std::vector<DevMatrix> mats_;
     std::vector<PagedCache> caches_;
+    std::vector<Buffer> spare_;  // freed blocks, oldest first
+    size_t spare_bytes_ = 0;
     float *kc_ = nullptr, *vc_ = nullptr;
     float *att_scratch_ = nullptr;
     size_t att_scratch_bytes_ = 0;

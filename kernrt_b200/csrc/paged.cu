@@ -13,18 +13,14 @@ cudaError_t launched() {
     return cudaGetLastError();
 }
 
-// One CTA per sequence: its descriptor and the table entries that changed;
-// the items are shared out over the CTAs.
-__global__ void __launch_bounds__(128) k_pages_step(const StepSeq *__restrict__ staged, int n_items,
-                                                    StepSeq *__restrict__ seqs, AttnItem *__restrict__ items,
+// One CTA per sequence: its descriptor, and the table entries that changed.
+__global__ void __launch_bounds__(128) k_pages_step(const StepSeq *__restrict__ staged, StepSeq *__restrict__ seqs,
                                                     int32_t *__restrict__ table, int max_pages) {
     const StepSeq q = staged[blockIdx.x];
-    const AttnItem *from = reinterpret_cast<const AttnItem *>(staged + gridDim.x);
-    const int32_t *delta = reinterpret_cast<const int32_t *>(from + n_items) + q.delta;
+    const int32_t *delta = reinterpret_cast<const int32_t *>(staged + gridDim.x) + q.delta;
     if (threadIdx.x == 0) seqs[blockIdx.x] = q;
     for (int i = threadIdx.x; i < q.n_dirty; i += blockDim.x)
         table[(size_t)q.slot * max_pages + q.dirty + i] = delta[i];
-    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n_items; i += gridDim.x * blockDim.x) items[i] = from[i];
 }
 
 // Eight elements of a k or v row per thread; the row's page comes from the
@@ -413,10 +409,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
 
 }  // namespace
 
-cudaError_t launch_pages_step(const StepSeq *staged, int n, int n_items, StepSeq *seqs, AttnItem *items,
-                              int32_t *table, int max_pages, cudaStream_t s) {
+cudaError_t launch_pages_step(const StepSeq *staged, int n, StepSeq *seqs, int32_t *table, int max_pages,
+                              cudaStream_t s) {
     if (n == 0) return cudaSuccess;
-    k_pages_step<<<(unsigned)n, 128, 0, s>>>(staged, n_items, seqs, items, table, max_pages);
+    k_pages_step<<<(unsigned)n, 128, 0, s>>>(staged, seqs, table, max_pages);
     return launched();
 }
 

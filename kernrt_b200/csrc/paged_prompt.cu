@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     using S = Shape<D, F32>;
     constexpr int Keys = S::Keys, W = S::Wide;
     extern __shared__ unsigned char raw_smem[];
-    __shared__ uint64_t slot_full[S::Slots], slot_empty[S::Slots], s_full[3], p_full[2], o_full[2], o_free, q_full, done, turn[2][4];
+    __shared__ uint64_t slot_full[S::Slots], slot_empty[S::Slots], s_full[3], p_full[2], o_full[2], o_free, q_full, done;
     __shared__ uint32_t s_tmem, s_red[2][4][2];
     __shared__ float s_kscale[kScaleRing], s_vscale[kScaleRing];
     __shared__ int s_abort, s_wild;
@@ -326,7 +326,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             mbar_init(&o_full[t], 1);
         }
         mbar_init(&o_free, 4);
-        for (int w = 0; w < 8; ++w) mbar_init(&turn[w >> 2][w & 3], 1);
         mbar_init(&q_full, 8);
         mbar_init(&done, 1);
         s_abort = 0;
@@ -482,14 +481,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 for (int d = 0; d < D / 2; ++d) acc[d] = mul2(acc[d], both(keep));
             }
             m = mn;
-            // The exponentials of warp w of both query tiles share one pair of
-            // units (16 a cycle and SM); taken in turns, each runs under the other's
-            // remaining work, where both at once would leave the units idle after.
-            const bool paired = n1 > 0 && tile < n0;
-            if (paired && t + tile > 0) {
-                ok = __all_sync(0xffffffffu, wait(&turn[t][warp & 3], (uint32_t)(tile - 1 + t) & 1u));
-                if (!ok) break;
-            }
             // weights times 2^14: the halves of small ones stay normal numbers
             const float bias = 14.0f - (m == -INFINITY ? 0.0f : m);
             F2 sum[2] = {both(0.0f), both(0.0f)};
@@ -516,8 +507,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             };
             if (masked) weights(Tile<1>{});
             else weights(Tile<0>{});
-            __syncwarp();
-            if (paired && lane == 0) mbar_arrive(&turn[t ^ 1][warp & 3]);
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
@@ -684,7 +673,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 if (!elect_one()) return;
                 const uint32_t a = here(k_desc(base + t * S::QTile)), k = here(k_desc(slots + slot * S::Slot));
                 const uint32_t d_at = here(tmem + buf * Keys);
-#pragma unroll
+#pragma unroll 1
                 for (int x = 0; x < S::Parts + 1; ++x) {  // q_hi K_hi, q_lo K_hi, q_hi K_lo
                     const int qo = x == 1 ? (D / 64) * 16384 : 0, ko = x == 2 ? (D / 64) * S::Sub : 0;
 #pragma unroll
@@ -698,7 +687,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 if (!elect_one()) return;
                 const uint32_t v = here(mn_desc(slots + slot * S::Slot, S::Sub)), w = here(tmem + buf * Keys);
                 const uint32_t d_at = here(tmem + S::SumAt + (S::Sums == 2 ? t * D : 0));
-#pragma unroll
+#pragma unroll 1
                 for (int x = 0; x < S::Parts + 1; ++x) {  // w_hi V_hi, w_lo V_hi, w_hi V_lo
                     const int vo = x == 2 ? (D / 64) * S::Sub : 0;
 #pragma unroll

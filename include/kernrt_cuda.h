@@ -470,7 +470,8 @@ int kernrt_cuda_pages_attention(kernrt_cuda_ctx *ctx, kernrt_pages pages, size_t
  * probabilities with their token ids, equal values by ascending id
  * (top_ids int32 and top_logprobs f32 [rows, top]).  targets and logprob, entropy,
  * and the top entries (top = 0) may each be left out with 0 handles; top is at
- * most KERNRT_TOP_MAX and at most vocab.  Outputs are buffers of their own.
+ * most KERNRT_TOP_MAX and at most vocab, vocab at most 2^24.  Outputs are buffers
+ * of their own.
  * Logits of -inf have probability 0.  A row holding NaN or +inf, or only -inf,
  * has no distribution: its outputs are NaN (its top ids still ordered by value,
  * NaN first).  A target outside the vocabulary gives NaN and KERNRT_E_DEVICE at

@@ -94,6 +94,7 @@ public:
         cudaFree(vc_);
         cudaFree(att_scratch_);
         for (auto &c : caches_) free_cache(c);
+        for (Grown *g : {&lp_parts_, &lp_lists_, &lp_count_}) cudaFree(g->ptr);
         drop_spare(0);
         cudaFree(d_err_);
         cudaFree(d_ticket_);
@@ -1751,7 +1752,7 @@ public:
     // ---- log probabilities of given tokens (logprobs.cu) ------------------------
     void logprobs(kernrt_buf logits, size_t rows, size_t vocab, kernrt_buf targets, kernrt_buf logprob,
                   kernrt_buf entropy, size_t top, kernrt_buf top_ids, kernrt_buf top_logprobs) {
-        if (vocab == 0 || vocab > (size_t)INT32_MAX / 2) fail(KERNRT_E_INVALID, "logprobs: bad vocabulary size");
+        if (vocab == 0 || vocab > ((size_t)1 << 24)) fail(KERNRT_E_INVALID, "logprobs: bad vocabulary size");
         if (top > KERNRT_TOP_MAX || top > vocab) fail(KERNRT_E_INVALID, "logprobs: too many top entries");
         if ((targets != 0) != (logprob != 0)) fail(KERNRT_E_INVALID, "logprobs: targets and logprob come together");
         if (top ? !top_ids || !top_logprobs : top_ids || top_logprobs)
@@ -1772,8 +1773,18 @@ public:
         flush();
         auto ints = [&](kernrt_buf h) { return h ? reinterpret_cast<int32_t *>(buf(h).ptr) : nullptr; };
         auto floats = [&](kernrt_buf h) { return h ? f(buf(h)) : nullptr; };
+        static_assert(kTopMost == KERNRT_TOP_MAX, "one limit");
+        const size_t chunks = rows ? (size_t)logprobs_chunks((int)rows, (int)vocab) : 0;
+        fits_int(rows * chunks, "logprobs");
+        if (chunks > 1) {
+            grow(lp_parts_, rows * chunks * 16);
+            grow(lp_lists_, rows * chunks * top * 8);
+            if (grow(lp_count_, rows * sizeof(unsigned)))
+                check(cudaMemsetAsync(lp_count_.ptr, 0, lp_count_.bytes, stream_), "cudaMemset");
+        }
         launch_or_fail(launch_logprobs(f(xb), (int)rows, (int)vocab, ints(targets), floats(logprob), floats(entropy),
-                                       (int)top, ints(top_ids), floats(top_logprobs), d_err_, stream_),
+                                       (int)top, ints(top_ids), floats(top_logprobs), lp_parts_.ptr, lp_lists_.ptr,
+                                       static_cast<unsigned *>(lp_count_.ptr), d_err_, stream_),
                        "logprobs");
     }
 
@@ -2175,6 +2186,7 @@ private:
     std::vector<Pending> pending_;
     std::vector<DevMatrix> mats_;
     std::vector<PagedCache> caches_;
+    Grown lp_parts_, lp_lists_, lp_count_;  // logprobs' scratch
     std::vector<Buffer> spare_;  // freed blocks, oldest first
     size_t spare_bytes_ = 0;
     float *kc_ = nullptr, *vc_ = nullptr;

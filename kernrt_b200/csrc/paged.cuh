@@ -75,7 +75,13 @@ cudaError_t launch_pages_prompt(const PagesView &p, int layer, const StepSeq *se
 
 // Per row of x [rows, vocab]: the target's log probability, the entropy, and
 // the `top` largest (ids ascending among equals) with their log probabilities.
+// Rows of more than one chunk take scratch: `parts` 16 bytes and `lists` 8 top
+// bytes for each of rows * logprobs_chunks(rows, vocab), and `count`, rows
+// counters that are 0 between launches.
+constexpr int kTopMost = 64;
+int logprobs_chunks(int rows, int vocab);
 cudaError_t launch_logprobs(const float *x, int rows, int vocab, const int32_t *targets, float *logprob,
-                            float *entropy, int top, int32_t *top_ids, float *top_logprobs, int *err, cudaStream_t s);
+                            float *entropy, int top, int32_t *top_ids, float *top_logprobs, void *parts, void *lists,
+                            unsigned *count, int *err, cudaStream_t s);
 
 }  // namespace krt

@@ -99,6 +99,17 @@ def test_sorted_rows(gpu, vocab):
     check(gpu, x, [0, vocab - 1, at], 64)
 
 
+def test_large_entries_spread_evenly_over_a_row(gpu):
+    """Every stretch of the row holds one entry less than `top` of the largest, so
+    that no stretch's list says much about the others'."""
+    rng = np.random.default_rng(12)
+    for vocab, every in ((151936, 1024), (600000, 1024), (600001, 2048)):
+        x = rng.standard_normal((1, vocab)).astype(np.float32)
+        at = np.arange(0, vocab - 64, every)[:, None] + np.arange(63)
+        x[0, at.ravel()] = 100 + rng.permutation(at.size).astype(np.float32) / 64
+        check(gpu, x, [5], 64)
+
+
 def test_masked_rows_and_rows_without_a_distribution(gpu):
     rng = np.random.default_rng(3)
     x = (3 * rng.standard_normal((9, 3001))).astype(np.float32)

@@ -234,6 +234,8 @@ class CudaBackend:
         _ok(self._lib.kernrt_cuda_create(int(device), C.byref(ctx)))
         self._ctx = ctx
         self._lens: dict[int, int] = {}
+        room = np.empty(1024, np.int32)
+        self._room = (room, _ptr(room), (SZ * 1)())  # where seq_table reads to
 
     # -- lifecycle ----------------------------------------------------------------
     def close(self) -> None:
@@ -530,11 +532,13 @@ class CudaBackend:
 
     def seq_table(self, pages: int, seq: int) -> np.ndarray:
         """The ids of the sequence's pages (int32)."""
-        n = SZ()
-        _ok(self._lib.kernrt_cuda_seq_table(self._ctx, pages, seq, None, None, 0, C.byref(n)))
-        out = np.empty(n.value, np.int32)
-        _ok(self._lib.kernrt_cuda_seq_table(self._ctx, pages, seq, None, _ptr(out), out.size, None))
-        return out
+        room, at, n = self._room
+        _ok(self._lib.kernrt_cuda_seq_table(self._ctx, pages, seq, None, at, room.size, n))
+        if n[0] > room.size:
+            room = np.empty(2 * n[0], np.int32)
+            self._room = (room, _ptr(room), n)
+            return self.seq_table(pages, seq)
+        return room[:n[0]].copy()
 
     def pages_compact(self, pages: int) -> int:
         """Moves the pages in use to the front of the pool; returns how many moved."""

@@ -1673,7 +1673,6 @@ public:
         std::vector<PageCopy> copies;
         paging([&] { c.map->extend(seqs, rows, n, &copies); });
         c.stepped = false;
-        copy_pages(c, copies);
         std::vector<StepSeq> desc;
         std::vector<int32_t> delta;
         size_t row0 = 0;
@@ -1696,13 +1695,20 @@ public:
         c.rows = row0;
         c.planned = false;
         if (!desc.empty()) {
+            // one upload: the descriptors, the tables' changes, the copies of
+            // shared pages
             const size_t a = desc.size() * sizeof(StepSeq), b = delta.size() * sizeof(int32_t);
-            std::vector<char> block(a + b);
+            std::vector<char> block(a + b + copies.size() * sizeof(CopyItem));
             std::memcpy(block.data(), desc.data(), a);
             if (b) std::memcpy(block.data() + a, delta.data(), b);
-            const auto *d = static_cast<const StepSeq *>(stage(block.data(), block.size()));
-            launch_or_fail(launch_pages_step(d, (int)desc.size(), c.seqs, c.table, c.view.max_pages, stream_),
+            if (!copies.empty()) std::memcpy(block.data() + a + b, copies.data(), copies.size() * sizeof(CopyItem));
+            const char *d = static_cast<const char *>(stage(block.data(), block.size()));
+            launch_or_fail(launch_pages_step(reinterpret_cast<const StepSeq *>(d), (int)desc.size(), c.seqs, c.table,
+                                             c.view.max_pages, stream_),
                            "pages_step");
+            launch_or_fail(launch_pages_copy(c.view, reinterpret_cast<const CopyItem *>(d + a + b), (int)copies.size(),
+                                             stream_),
+                           "pages_step (copies)");
             for (const StepSeq &q : desc) c.map->at((size_t)q.slot).dirty = c.map->at((size_t)q.slot).pages.size();
         }
         c.step = std::move(desc);

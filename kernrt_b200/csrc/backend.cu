@@ -1560,14 +1560,7 @@ public:
     static AttnPlan plan_attention(const PagesView &v, const std::vector<StepSeq> &desc) {
         AttnPlan a;
         const size_t sms = (size_t)device_sms(), hk = (size_t)v.kv_heads;
-        size_t keys = 0;
-        for (const StepSeq &d : desc)
-            if (d.rows * v.group <= kFewRows)
-                keys += (size_t)((d.rows * v.group + kDecodeRows - 1) / kDecodeRows) * (size_t)(d.ctx + d.rows);
-        // pieces of about as many keys as fill every SM four times, and of at
-        // most 1024, so that a warp sums no more than 256 keys in a row
-        const size_t share = std::min<size_t>(1024, keys * hk / (4 * sms) + 1);
-        const int cut = (int)((share + kDecodeKeys - 1) / kDecodeKeys * kDecodeKeys);
+        const int cut = decode_cut(v, desc, sms, hk);
         for (size_t i = 0; i < desc.size(); ++i) {
             const StepSeq &d = desc[i];
             const int m = d.rows * v.group;
@@ -1592,6 +1585,35 @@ public:
         for (size_t i = 0; i < a.prompt.size(); ++i) a.prompt[i].first = (int32_t)i;
         split_prompts(a, sms, hk);
         return a;
+    }
+
+    // The length of the single tokens' pieces.  Of shares that fill the CTAs that
+    // run at once in 1, 2 .. rounds, the one that ends soonest: whole rounds of
+    // full pieces, or an even share and one piece over, whichever is less.  A
+    // piece's start and join cost about as much as 100 keys.
+    static int decode_cut(const PagesView &v, const std::vector<StepSeq> &desc, size_t sms, size_t hk) {
+        constexpr size_t kPieceCost = 100;
+        const auto groups = [&](const StepSeq &d) {
+            const int m = d.rows * v.group;
+            return m <= kFewRows ? (size_t)((m + kDecodeRows - 1) / kDecodeRows) : 0;
+        };
+        size_t keys = 0;
+        for (const StepSeq &d : desc) keys += groups(d) * (size_t)(d.ctx + d.rows);
+        if (keys == 0) return kDecodeKeys;
+        const size_t slots = sms * (size_t)pages_decode_ctas(v);
+        size_t best = 0, best_cost = 0;
+        for (size_t rounds : {1, 2, 3, 4, 6, 8}) {
+            const size_t share = keys * hk / (slots * rounds) + 1;
+            const size_t cut = std::min<size_t>((share + kDecodeKeys - 1) / kDecodeKeys * kDecodeKeys, 1u << 20);
+            size_t pieces = 0;
+            for (const StepSeq &d : desc) pieces += groups(d) * (((size_t)(d.ctx + d.rows) + cut - 1) / cut);
+            pieces *= hk;
+            const size_t whole = (pieces + slots - 1) / slots * (cut + kPieceCost);
+            const size_t even = (keys * hk + pieces * kPieceCost) / slots + cut + kPieceCost;
+            const size_t cost = std::min(whole, even);
+            if (best == 0 || cost < best_cost) best = cut, best_cost = cost;
+        }
+        return (int)best;
     }
 
     // Few and long pieces (a chunk behind a long context) are cut so that they

@@ -4,6 +4,8 @@
 #include "paged.cuh"
 #include "paged_dev.cuh"
 
+#include <type_traits>
+
 namespace krt {
 
 namespace {
@@ -86,12 +88,16 @@ __global__ void __launch_bounds__(256) k_pages_copy(PagesView p, const CopyItem 
 
 // ---- single tokens: attention split over the length ------------------------------
 //
-// One warp takes 16 positions at a time against 8 query rows with m16n8k16 MMAs
-// whose operands it loads straight into registers.  A product over k or over
-// the keys may take its terms in any order, so each thread reads 16 contiguous
-// bytes and the fragments follow from that: for scores, thread (g, t) = (lane /
-// 4, lane % 4) holds elements 32 b + 8 t .. + 7 of key g; for values, elements 64
-// b + 8 g .. + 7 of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
+// One warp takes 16 positions at a time against 8 query rows with m16n8k16 MMAs.
+// Its tiles come through a ring in shared memory of its own (cp.async, no
+// barrier beyond the warp's), so that several are in flight while one is used.
+// A product over k or over the keys may take its terms in any order, so each
+// thread reads 16 contiguous bytes (32 of f32) and the fragments follow from
+// that: for scores, thread (g, t) = (lane / 4, lane % 4) holds elements 32 b + 8 t ..
+// + 7 of column g, which is key 8 u + 4 (g % 2) + g / 2 of the tile; for values,
+// elements 64 b + 8 g .. + 7 of keys t, t + 4, t + 8, t + 12, the ones whose weights
+// are in its registers.  A row's 16-byte chunks are swizzled (swap) so that the
+// eight lanes of a shared-memory access reach all banks.
 //
 // Precision: f32 queries and weights go in as three bf16 parts (24 bits: x = x1
 // + x2 + x3 with each part the rounding of what is left), which a bf16 cache
@@ -99,7 +105,10 @@ __global__ void __launch_bounds__(256) k_pages_copy(PagesView p, const CopyItem 
 // and 2 share one MMA (rows 0-7 and 8-15) and part 3 takes a second into the
 // accumulator of part 1; a thread then finds the parts of one score in its own
 // registers.  An f32 cache is split the same way, and the products down to
-// 2^-24 are kept: (x1 + x2) k1, x3 k1, (x1 + x2) k2, x1 k3.
+// 2^-24 are kept: (x1 + x2) k1, x3 k1, (x1 + x2) k2, x1 k3.  The MMAs add with
+// truncation, so after every 16 tiles the sums go to shared memory, where they
+// are added with rounding (added in registers after every tile, 64 x 8000 keys of
+// 16 heads of 128 took 207 us instead of 177).
 template <int NB>
 struct QFrag {  // [block of 32][half of it]: A of parts 1 and 2, and of part 3
     uint32_t a[NB][2][4], c[NB][2][2];
@@ -139,19 +148,34 @@ struct Chunk;
 template <>
 struct Chunk<false> {
     uint4 v;
-    __device__ __forceinline__ void load(const void *kv, size_t e, bool ok) {
-        v = ok ? __ldg(reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(kv) + e)) : make_uint4(0, 0, 0, 0);
+    __device__ __forceinline__ void load(const unsigned char *row, int c, int swap) {
+        v = *reinterpret_cast<const uint4 *>(row + ((c ^ swap) << 4));
     }
 };
 template <>
 struct Chunk<true> {
     float4 v[2];
-    __device__ __forceinline__ void load(const void *kv, size_t e, bool ok) {
-        const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(kv) + e);
-        const float4 z = make_float4(0, 0, 0, 0);
-        v[0] = ok ? __ldg(p) : z;
-        v[1] = ok ? __ldg(p + 1) : z;
+    __device__ __forceinline__ void load(const unsigned char *row, int c, int swap) {
+        v[0] = *reinterpret_cast<const float4 *>(row + (((2 * c) ^ swap) << 4));
+        v[1] = *reinterpret_cast<const float4 *>(row + (((2 * c + 1) ^ swap) << 4));
     }
+};
+template <bool F32>
+__device__ __forceinline__ int k_swap(int row) { return F32 ? row >> 2 & 1 : row & 7; }
+template <bool F32>
+__device__ __forceinline__ int v_swap(int row) { return F32 ? (row & 1) | (row & 2) << 1 : (row & 3) << 1; }
+
+// 16 bytes to shared memory, or zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+
+template <int NB, bool F32>
+struct Ring {
+    static constexpr int Row = F32 ? 128 * NB : 128 * ((NB + 1) / 2);  // bytes of a row
+    static constexpr int Tile = 16 * Row;                              // of K or V
+    static constexpr int Stages = Tile <= 2048 ? 4 : 3;
+    static constexpr int Bytes = Stages * 2 * Tile;                    // of a warp
 };
 
 constexpr int kDecodeWarps = 4;
@@ -162,6 +186,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
                    AttnScratch scratch, const float *__restrict__ q, float *__restrict__ out) {
     constexpr int NV = (NB + 1) / 2;  // blocks of 64 of the values
     constexpr int R = kDecodeRows;
+    using G = Ring<NB, F32>;
+    extern __shared__ __align__(128) unsigned char ring[];
     __shared__ float s_o[kDecodeWarps][R][32 * NB + 4];
     __shared__ float s_m[kDecodeWarps][R], s_l[kDecodeWarps][R];
     __shared__ int s_last;
@@ -204,48 +230,82 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
 #pragma unroll
             for (int x = 0; x < 4; ++x) o[b][i][x] = 0.0f;
     float m = -INFINITY, l = 0.0f;
+    // the sums so far to shared memory, relative to the maximum m_out (a thread's
+    // elements are its own there)
+    float m_out = -INFINITY;
+    const auto put_out = [&]() {
+        const float keep = m_out == -INFINITY ? 0.0f : ex2(m_out - m);
+#pragma unroll
+        for (int b = 0; b < NV; ++b)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int d = 64 * b + 8 * (2 * t + x) + i;
+                    if (d >= 32 * NB) continue;
+                    const float v = o[b][i][x] + o[b][i][2 + x];
+                    s_o[warp][g][d] = m_out == -INFINITY ? v : __fmaf_rn(s_o[warp][g][d], keep, v);
+                    o[b][i][x] = o[b][i][2 + x] = 0.0f;
+                }
+        m_out = m;
+    };
 
     // this warp's tiles: 16 positions at lo + 16 warp, step 64; a tile never
     // leaves its page
     const int t0 = it.lo + 16 * warp;
     const int n_tiles = it.hi > t0 ? (it.hi - t0 + kDecodeKeys - 1) / kDecodeKeys : 0;
+    unsigned char *const mine = ring + warp * G::Bytes;
+    const uint32_t mine_at = (uint32_t)__cvta_generic_to_shared(mine);
     int pages = 0;  // lane i: the page of tile i of the current 32
-    for (int tile = 0; tile < n_tiles; ++tile) {
-        if ((tile & 31) == 0) {
-            const int at = t0 + kDecodeKeys * (tile + lane);
-            pages = at < it.hi ? __ldg(table + (at >> p.page_shift)) : 0;
-        }
-        const int pos = t0 + kDecodeKeys * tile;
-        const size_t row0 = (size_t)__shfl_sync(0xffffffffu, pages, tile & 31) * page_stride +
-                            (size_t)(pos & page_mask) * head;
-        Chunk<F32> kc[2][NB], vc[NV][4];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-                kc[u][b].load(p.kv, k_base + row0 + (size_t)(8 * u + g) * head + 8 * (4 * b + t),
-                              4 * b + t < chunks && pos + 8 * u + g < it.hi);
-#pragma unroll
-        for (int b = 0; b < NV; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = 2 * t + (i & 1) + 8 * (i >> 1);
-                vc[b][i].load(p.kv, v_base + row0 + (size_t)key * head + 8 * (8 * b + g),
-                              8 * b + g < chunks && pos + key < it.hi);
+    const char *const kv = static_cast<const char *>(p.kv);
+    constexpr int Size = F32 ? 4 : 2, PerRow = G::Row / 16;  // chunks of a row in shared memory
+    const int have = head * Size / 16;                       // of them in a page
+    const auto fetch = [&](int tile) {
+        if (tile < n_tiles) {
+            if ((tile & 31) == 0) {
+                const int at = t0 + kDecodeKeys * (tile + lane);
+                pages = at < it.hi ? __ldg(table + (at >> p.page_shift)) : 0;
             }
+            const int pos = t0 + kDecodeKeys * tile;
+            const size_t row0 = (size_t)__shfl_sync(0xffffffffu, pages, tile & 31) * page_stride +
+                                (size_t)(pos & page_mask) * head;
+            const uint32_t to = mine_at + (uint32_t)(tile % G::Stages) * (2 * G::Tile);
+            const char *const k_src = kv + (k_base + row0) * Size, *const v_src = kv + (v_base + row0) * Size;
+#pragma unroll
+            for (int i = 0; i < PerRow / 2; ++i) {  // 16 rows of PerRow chunks
+                const int at = lane + 32 * i, r = at / PerRow, c = at % PerRow;
+                const bool in = c < have && pos + r < it.hi;
+                const size_t off = in ? (size_t)r * head * Size + 16 * c : 0;
+                copy16(to + r * G::Row + ((c ^ k_swap<F32>(r)) << 4), k_src + off, in);
+                copy16(to + G::Tile + r * G::Row + ((c ^ v_swap<F32>(r)) << 4), v_src + off, in);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < G::Stages - 1; ++i) fetch(i);
+    for (int tile = 0; tile < n_tiles; ++tile) {
+        const int pos = t0 + kDecodeKeys * tile;
+        asm volatile("cp.async.wait_group %0;" ::"n"(G::Stages - 2) : "memory");
+        __syncwarp();
+        fetch(tile + G::Stages - 1);  // into the place of the tile used last
+        const unsigned char *const k_tile = mine + (tile % G::Stages) * (2 * G::Tile), *const v_tile = k_tile + G::Tile;
 
         float s[2][2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const int key = 8 * u + 4 * (g & 1) + (g >> 1);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
+                Chunk<F32> kc;
+                kc.load(k_tile + key * G::Row, 4 * b + t, k_swap<F32>(key));
                 if constexpr (F32) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t k1[2], k2[2], k3[2];
-                        split3(kc[u][b].v[h].x, kc[u][b].v[h].y, k1[0], k2[0], k3[0]);
-                        split3(kc[u][b].v[h].z, kc[u][b].v[h].w, k1[1], k2[1], k3[1]);
+                        split3(kc.v[h].x, kc.v[h].y, k1[0], k2[0], k3[0]);
+                        split3(kc.v[h].z, kc.v[h].w, k1[1], k2[1], k3[1]);
                         const uint32_t(&a)[4] = qf.a[b][h];
                         mma16816(c, a[0], a[1], a[2], a[3], k1[0], k1[1]);
                         mma16816(c, a[0], a[1], a[2], a[3], k2[0], k2[1]);
@@ -253,7 +313,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
                         mma16816(c, qf.c[b][h][0], 0, qf.c[b][h][1], 0, k1[0], k1[1]);
                     }
                 } else {
-                    const uint32_t k[4] = {kc[u][b].v.x, kc[u][b].v.y, kc[u][b].v.z, kc[u][b].v.w};
+                    const uint32_t k[4] = {kc.v.x, kc.v.y, kc.v.z, kc.v.w};
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const uint32_t(&a)[4] = qf.a[b][h];
@@ -262,10 +322,11 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
                     }
                 }
             }
-            // rows 0-7 hold parts 1 and 3, rows 8-15 part 2 of the same score
-            const int at = pos + 8 * u + 2 * t;
+            // rows 0-7 hold parts 1 and 3, rows 8-15 part 2 of the same score;
+            // columns 2 t and 2 t + 1 are keys 8 u + t and 8 u + 4 + t
+            const int at = pos + 8 * u + t;
             s[u][0] = at < limit ? (c[0] + c[2]) * scale : -INFINITY;
-            s[u][1] = at + 1 < limit ? (c[1] + c[3]) * scale : -INFINITY;
+            s[u][1] = at + 4 < limit ? (c[1] + c[3]) * scale : -INFINITY;
         }
         float mt = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
@@ -293,12 +354,22 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
         }
 #pragma unroll
         for (int b = 0; b < NV; ++b) {
+            Chunk<F32> vc[4];  // (blocks past the row are not read)
+            if (F32 && 64 * b + 32 >= 32 * NB) {  // the row ends inside the block
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    if (g < 4) vc[x].load(v_tile + (4 * x + t) * G::Row, 8 * b + g, v_swap<F32>(t));
+                    else vc[x] = Chunk<F32>{};
+            } else {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) vc[x].load(v_tile + (4 * x + t) * G::Row, 8 * b + g, v_swap<F32>(t));
+            }
             if constexpr (F32) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     float e[4];
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) e[x] = (&vc[b][x].v[i >> 2].x)[i & 3];
+                    for (int x = 0; x < 4; ++x) e[x] = (&vc[x].v[i >> 2].x)[i & 3];
                     uint32_t v1[2], v2[2], v3[2];
                     split3(e[0], e[1], v1[0], v2[0], v3[0]);
                     split3(e[2], e[3], v1[1], v2[1], v3[1]);
@@ -311,13 +382,14 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const uint32_t sel = (i & 1) ? 0x7632u : 0x5410u;
-                    const uint32_t b0 = __byte_perm((&vc[b][0].v.x)[i >> 1], (&vc[b][1].v.x)[i >> 1], sel);
-                    const uint32_t b1 = __byte_perm((&vc[b][2].v.x)[i >> 1], (&vc[b][3].v.x)[i >> 1], sel);
+                    const uint32_t b0 = __byte_perm((&vc[0].v.x)[i >> 1], (&vc[1].v.x)[i >> 1], sel);
+                    const uint32_t b1 = __byte_perm((&vc[2].v.x)[i >> 1], (&vc[3].v.x)[i >> 1], sel);
                     mma16816(o[b][i], pa[0], pa[1], pa[2], pa[3], b0, b1);
                     mma16816(o[b][i], pc[0], 0, pc[1], 0, b0, b1);
                 }
             }
         }
+        if ((tile & 15) == 15) put_out();
     }
 
     // the CTA's warps meet in shared memory
@@ -327,15 +399,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
         s_m[warp][g] = m;
         s_l[warp][g] = l;
     }
-#pragma unroll
-    for (int b = 0; b < NV; ++b)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int d = 64 * b + 8 * (2 * t + x) + i;
-                if (d < 32 * NB) s_o[warp][g][d] = o[b][i][x] + o[b][i][2 + x];
-            }
+    put_out();
     __syncthreads();
     const size_t piece = (size_t)blockIdx.x * p.kv_heads + j;
     // warp w: rows w, w + 4; lane: elements lane + 32 i
@@ -390,30 +454,72 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
     __syncthreads();
     if (!s_last) return;
     __threadfence();
+    // The ring's memory is free: the pieces' weights 2^(m_i - M), Batch of each row
+    // at a time, and the sums of the threads that share four elements.
+    constexpr int Batch = 512, Threads = 32 * kDecodeWarps;
+    float *const weight = reinterpret_cast<float *>(ring);                 // [R][Batch]
+    float4 *const sums = reinterpret_cast<float4 *>(weight + R * Batch);   // [units]
+    const size_t first = ((size_t)it.first * p.kv_heads + j) * R, step = (size_t)p.kv_heads * R;
     for (int r = warp; r < it.rows; r += kDecodeWarps) {
-        const size_t first = ((size_t)it.first * p.kv_heads + j) * R + r, step = (size_t)p.kv_heads * R;
         float M = -INFINITY;
-        for (int i = lane; i < it.n_parts; i += 32) M = fmaxf(M, __ldcg(&scratch.ml[first + i * step]).x);
+#pragma unroll 4
+        for (int i = lane; i < it.n_parts; i += 32) M = fmaxf(M, __ldcg(&scratch.ml[first + r + i * step]).x);
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-        float L = 0.0f, acc[NB];
+        if (lane == 0) s_m[0][r] = M, s_l[0][r] = 0.0f;
+    }
+    __syncwarp();
+    const int quads = head >> 2, groups = it.rows * quads, shares = max(1, Threads / groups);
+    constexpr int Units = R * kHeadMax / 4 / Threads;  // at most, of a thread
+    float4 acc[Units];
 #pragma unroll
-        for (int i = 0; i < NB; ++i) acc[i] = 0.0f;
-#pragma unroll 4
-        for (int i = 0; i < it.n_parts; ++i) {
-            const size_t w = first + i * step;
-            const float2 ml = __ldcg(&scratch.ml[w]);
-            const float k = M == -INFINITY ? 0.0f : ex2(ml.x - M);
-            L = __fmaf_rn(ml.y, k, L);
+    for (int x = 0; x < Units; ++x) acc[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int base = 0; base < it.n_parts; base += Batch) {
+        const int n = min(Batch, it.n_parts - base);
+        for (int r = warp; r < it.rows; r += kDecodeWarps) {
+            const float M = s_m[0][r];
+            float L = 0.0f;
+            for (int i = lane; i < n; i += 32) {
+                const float2 ml = __ldcg(&scratch.ml[first + r + (base + i) * step]);
+                const float k = M == -INFINITY ? 0.0f : ex2(ml.x - M);
+                weight[r * Batch + i] = k;
+                L = __fmaf_rn(ml.y, k, L);
+            }
 #pragma unroll
-            for (int x = 0; x < NB; ++x)
-                if (lane + 32 * x < head) acc[x] = __fmaf_rn(__ldcg(&scratch.o[w * head + lane + 32 * x]), k, acc[x]);
+            for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
+            if (lane == 0) s_l[0][r] += L;
         }
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < Units; ++x) {
+            const int u = threadIdx.x + x * Threads, group = u % groups, r = group / quads;
+            if (u >= groups * shares) break;
+            const float4 *src = reinterpret_cast<const float4 *>(scratch.o + (first + r + base * step) * head) + group % quads;
+#pragma unroll 8
+            for (int i = u / groups; i < n; i += shares) {
+                const float4 v = __ldcg(src + i * step * quads);
+                const float k = weight[r * Batch + i];
+                acc[x] = make_float4(__fmaf_rn(v.x, k, acc[x].x), __fmaf_rn(v.y, k, acc[x].y),
+                                     __fmaf_rn(v.z, k, acc[x].z), __fmaf_rn(v.w, k, acc[x].w));
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int x = 0; x < Units; ++x)
+        if (threadIdx.x + x * Threads < groups * shares) sums[threadIdx.x + x * Threads] = acc[x];
+    __syncthreads();
+    for (int group = threadIdx.x; group < groups; group += Threads) {
+        const int r = group / quads;
+        float4 v = sums[group];
+        for (int i = 1; i < shares; ++i) {
+            const float4 w = sums[group + i * groups];
+            v = make_float4(v.x + w.x, v.y + w.y, v.z + w.z, v.w + w.w);
+        }
+        const float L = s_l[0][r];
         const int mr = it.row + r, tok = mr / p.group;
         const size_t at = ((size_t)(sq.row0 + tok) * p.heads + (size_t)j * p.group + (mr - tok * p.group)) * head;
-#pragma unroll
-        for (int x = 0; x < NB; ++x)
-            if (lane + 32 * x < head) out[at + lane + 32 * x] = acc[x] / L;
+        reinterpret_cast<float4 *>(out + at)[group % quads] = make_float4(v.x / L, v.y / L, v.z / L, v.w / L);
     }
 }
 
@@ -446,24 +552,65 @@ cudaError_t launch_pages_copy(const PagesView &p, const CopyItem *items, int n, 
     return launched();
 }
 
+namespace {
+
+// Calls f(NB, F32) with the cache's head blocks and kind as types.
+template <class F>
+auto by_shape(const PagesView &p, F &&f) {
+    const auto by_head = [&](auto f32) {
+        switch ((p.head + 31) / 32) {
+        case 1: return f(std::integral_constant<int, 1>{}, f32);
+        case 2: return f(std::integral_constant<int, 2>{}, f32);
+        case 3: return f(std::integral_constant<int, 3>{}, f32);
+        default: return f(std::integral_constant<int, 4>{}, f32);
+        }
+    };
+    return p.f32 ? by_head(std::true_type{}) : by_head(std::false_type{});
+}
+
+// Opts k_pages_decode into its shared memory on the current device; returns its
+// CTAs per SM in *ctas.
+template <int NB, bool F32>
+cudaError_t decode_ready(int *ctas) {
+    static int known[64] = {0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) dev = 0;
+    if (known[dev] == 0) {
+        constexpr int smem = kDecodeWarps * Ring<NB, F32>::Bytes;
+        cudaError_t e = cudaFuncSetAttribute(k_pages_decode<NB, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        int n = 0;
+        if (e == cudaSuccess)
+            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_pages_decode<NB, F32>, 32 * kDecodeWarps, smem);
+        if (e != cudaSuccess) return e;
+        known[dev] = n > 0 ? n : 1;
+    }
+    *ctas = known[dev];
+    return cudaSuccess;
+}
+
+}  // namespace
+
+int pages_decode_ctas(const PagesView &p) {
+    int n = 1;
+    by_shape(p, [&](auto nb, auto f32) { return decode_ready<decltype(nb)::value, decltype(f32)::value>(&n); });
+    return n;
+}
+
 cudaError_t launch_pages_decode(const PagesView &p, int layer, const StepSeq *seqs, const AttnItem *items, int n_items,
                                 const AttnScratch &scratch, const float *q, float *out, cudaStream_t s) {
     if (n_items == 0) return cudaSuccess;
     const dim3 grid((unsigned)n_items, (unsigned)p.kv_heads);
-    const auto go = [&](auto kernel) { kernel<<<grid, 32 * kDecodeWarps, 0, s>>>(p, layer, seqs, items, scratch, q, out); };
-    const int nb = (p.head + 31) / 32;
-    if (p.f32) {
-        if (nb == 1) go(k_pages_decode<1, true>);
-        else if (nb == 2) go(k_pages_decode<2, true>);
-        else if (nb == 3) go(k_pages_decode<3, true>);
-        else go(k_pages_decode<4, true>);
-    } else {
-        if (nb == 1) go(k_pages_decode<1, false>);
-        else if (nb == 2) go(k_pages_decode<2, false>);
-        else if (nb == 3) go(k_pages_decode<3, false>);
-        else go(k_pages_decode<4, false>);
-    }
-    return launched();
+    return by_shape(p, [&](auto nb, auto f32) {
+        constexpr int NB = decltype(nb)::value;
+        constexpr bool F32 = decltype(f32)::value;
+        int n = 0;
+        const cudaError_t e = decode_ready<NB, F32>(&n);
+        if (e != cudaSuccess) return e;
+        k_pages_decode<NB, F32><<<grid, 32 * kDecodeWarps, kDecodeWarps * Ring<NB, F32>::Bytes, s>>>(
+            p, layer, seqs, items, scratch, q, out);
+        return launched();
+    });
 }
 
 }  // namespace krt

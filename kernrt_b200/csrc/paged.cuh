@@ -65,6 +65,8 @@ constexpr int kDecodeKeys = 64;  // positions a CTA takes at once: what splits a
 cudaError_t launch_pages_decode(const PagesView &p, int layer, const StepSeq *seqs, const AttnItem *items, int n_items,
                                 const AttnScratch &scratch, const float *q, float *out, cudaStream_t s);
 
+int pages_decode_ctas(const PagesView &p);  // CTAs an SM runs at once
+
 // The same for pieces of many rows (paged_prompt.cu); `split`: some piece has
 // more than one part.
 constexpr int kPromptRows = 256;

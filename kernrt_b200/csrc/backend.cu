@@ -1547,28 +1547,42 @@ public:
         return moves.size();
     }
 
-    // The step's attention cut into pieces.  A sequence with at most
-    // kFewRows query rows per kv head goes to the kernel for single tokens (groups
-    // of 8 rows that each read the keys again), one with more to the tensor
-    // cores' (256 rows; a piece costs 128 or more whatever it holds).
+    // The step's attention cut into pieces.  A sequence with at most kFewRows
+    // query rows per kv head goes to the kernel for single tokens (groups of 8
+    // rows that each read the keys again), and so do all where the rest is little
+    // work for it: the tensor cores' kernel (256 rows a piece) takes 15 to 40 us
+    // whatever it is given (128 tokens of 9 heads of 64: 11.3 against 17.5 us; 32
+    // behind 1000, 16 heads of 128: 21 against 38; 32 behind 8000: 55 against 44;
+    // 16 behind 8000: 30 against 38, in f32 pages 71 against 46).
     struct AttnPlan {
         std::vector<AttnItem> decode, prompt;
         size_t decode_parts = 0, joins = 0, prompt_parts = 0;
     };
     static constexpr int kFewRows = 16;
+    static constexpr size_t kFewWork = 36u << 20;  // groups of 8 rows x keys x head, x 2.5 for f32 pages
+
+    static bool few_rows(const PagesView &v, const StepSeq &d) { return d.rows * v.group <= kFewRows; }
+    static size_t row_groups(const PagesView &v, const StepSeq &d) {
+        return ((size_t)d.rows * v.group + kDecodeRows - 1) / kDecodeRows;
+    }
 
     static AttnPlan plan_attention(const PagesView &v, const std::vector<StepSeq> &desc) {
         AttnPlan a;
         const size_t sms = (size_t)device_sms(), hk = (size_t)v.kv_heads;
-        const int cut = decode_cut(v, desc, sms, hk);
+        size_t rest = 0;
+        for (const StepSeq &d : desc)
+            if (!few_rows(v, d)) rest += row_groups(v, d) * (size_t)(d.ctx + d.rows / 2 + 1) * hk * (size_t)v.head;
+        const bool all = rest * (v.f32 ? 5 : 2) / 2 <= kFewWork;
+        const int cut = decode_cut(v, desc, all, sms, hk);
         for (size_t i = 0; i < desc.size(); ++i) {
             const StepSeq &d = desc[i];
             const int m = d.rows * v.group;
-            const int step = m <= kFewRows ? kDecodeRows : kPromptRows;
+            const bool few = all || few_rows(v, d);
+            const int step = few ? kDecodeRows : kPromptRows;
             for (int row = 0; row < m; row += step) {
                 const int rows = std::min(step, m - row);
                 const int hi = d.ctx + (row + rows - 1) / v.group + 1;
-                if (m > kFewRows) {
+                if (!few) {
                     a.prompt.push_back({(int32_t)i, row, rows, 0, hi, 0, 1, 0});
                     continue;
                 }
@@ -1591,12 +1605,9 @@ public:
     // run at once in 1, 2 .. rounds, the one that ends soonest: whole rounds of
     // full pieces, or an even share and one piece over, whichever is less.  A
     // piece's start and join cost about as much as 100 keys.
-    static int decode_cut(const PagesView &v, const std::vector<StepSeq> &desc, size_t sms, size_t hk) {
+    static int decode_cut(const PagesView &v, const std::vector<StepSeq> &desc, bool all, size_t sms, size_t hk) {
         constexpr size_t kPieceCost = 100;
-        const auto groups = [&](const StepSeq &d) {
-            const int m = d.rows * v.group;
-            return m <= kFewRows ? (size_t)((m + kDecodeRows - 1) / kDecodeRows) : 0;
-        };
+        const auto groups = [&](const StepSeq &d) { return all || few_rows(v, d) ? row_groups(v, d) : 0; };
         size_t keys = 0;
         for (const StepSeq &d : desc) keys += groups(d) * (size_t)(d.ctx + d.rows);
         if (keys == 0) return kDecodeKeys;

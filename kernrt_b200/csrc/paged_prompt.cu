@@ -384,16 +384,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         {  // the row's halves, scaled to its largest element
             const int chunks = p.head >> 3;
             const float4 *src = reinterpret_cast<const float4 *>(q + at);
+            float4 x[D / 4];  // (the registers of acc)
+#pragma unroll
+            for (int c = 0; c < D / 4; ++c)
+                x[c] = live && c < 2 * chunks ? __ldg(src + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             uint32_t most = 0, least = 0xffffffffu;
-#pragma unroll 4
+#pragma unroll
             for (int c = 0; c < D / 8; ++c) {
-                if (!live || c >= chunks) break;
-                const float4 a = __ldg(src + 2 * c), b = __ldg(src + 2 * c + 1);
-                const float x = fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w)));
-                const float y = fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w)));
-                uint32_t m = __float_as_uint(fmaxf(x, y));
-                const float z = ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
-                if (z != z) m = 0x7f800000u;  // NaN, or infinities of both signs
+                const float4 a = x[2 * c], b = x[2 * c + 1];
+                const uint32_t m = max(max(max(__float_as_uint(fabsf(a.x)), __float_as_uint(fabsf(a.y))),
+                                           max(__float_as_uint(fabsf(a.z)), __float_as_uint(fabsf(a.w)))),
+                                       max(max(__float_as_uint(fabsf(b.x)), __float_as_uint(fabsf(b.y))),
+                                           max(__float_as_uint(fabsf(b.z)), __float_as_uint(fabsf(b.w)))));
                 most = max(most, m);
                 least = min(least, m - 1);
             }
@@ -401,15 +403,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             const float up = up_scale(most);
             sc = kLog2e * rsqrtf((float)p.head) * down_scale(up);
             const uint32_t tile = base + (uint32_t)t * S::QTile;
-#pragma unroll 2
+#pragma unroll
             for (int c = 0; c < D / 8; ++c) {
-                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
-                if (live && c < chunks) {
-                    x = __ldg(src + 2 * c);
-                    y = __ldg(src + 2 * c + 1);
-                }
                 uint4 hi, lo;
-                halves(x, y, up, hi, lo);
+                halves(x[2 * c], x[2 * c + 1], up, hi, lo);
                 const uint32_t o = tile + (uint32_t)(c >> 3) * 16384 + swizzled(r & 127, c & 7);
                 store_shared(o, hi);
                 store_shared(o + (D / 64) * 16384, lo);

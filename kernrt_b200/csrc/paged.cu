@@ -30,6 +30,7 @@ __global__ void __launch_bounds__(128) k_pages_step(const StepSeq *__restrict__ 
 __global__ void __launch_bounds__(256) k_pages_write(PagesView p, int layer, const StepSeq *__restrict__ seqs, int n,
                                                      int rows, const float4 *__restrict__ k,
                                                      const float4 *__restrict__ v) {
+    let_next_start();
     const int row_chunks = p.kv_heads * p.head / 8, head_chunks = p.head / 8;
     const size_t total = (size_t)rows * 2 * row_chunks;
     for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < total; i += (size_t)gridDim.x * blockDim.x) {
@@ -206,6 +207,17 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
     const int limit = live ? min(it.hi, sq.ctx + token + 1) : 0;
     const size_t q_at = ((size_t)(sq.row0 + token) * p.heads + (size_t)j * p.group + (m_row - token * p.group)) * head;
 
+    // this warp's tiles: 16 positions at lo + 16 warp, step 64; a tile never
+    // leaves its page
+    const int t0 = it.lo + 16 * warp;
+    const int n_tiles = it.hi > t0 ? (it.hi - t0 + kDecodeKeys - 1) / kDecodeKeys : 0;
+    const auto page_ids = [&](int tile) {  // lane i: the page of tile + i
+        const int at = t0 + kDecodeKeys * (tile + lane);
+        return at < it.hi ? __ldg(table + (at >> p.page_shift)) : 0;
+    };
+    int pages = page_ids(0);  // of the current 32 tiles
+    wait_before();
+
     QFrag<NB> qf;
     const float scale = kLog2e * rsqrtf((float)head);
 #pragma unroll
@@ -250,22 +262,14 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
         m_out = m;
     };
 
-    // this warp's tiles: 16 positions at lo + 16 warp, step 64; a tile never
-    // leaves its page
-    const int t0 = it.lo + 16 * warp;
-    const int n_tiles = it.hi > t0 ? (it.hi - t0 + kDecodeKeys - 1) / kDecodeKeys : 0;
     unsigned char *const mine = ring + warp * G::Bytes;
     const uint32_t mine_at = (uint32_t)__cvta_generic_to_shared(mine);
-    int pages = 0;  // lane i: the page of tile i of the current 32
     const char *const kv = static_cast<const char *>(p.kv);
     constexpr int Size = F32 ? 4 : 2, PerRow = G::Row / 16;  // chunks of a row in shared memory
     const int have = head * Size / 16;                       // of them in a page
     const auto fetch = [&](int tile) {
         if (tile < n_tiles) {
-            if ((tile & 31) == 0) {
-                const int at = t0 + kDecodeKeys * (tile + lane);
-                pages = at < it.hi ? __ldg(table + (at >> p.page_shift)) : 0;
-            }
+            if ((tile & 31) == 0 && tile > 0) pages = page_ids(tile);
             const int pos = t0 + kDecodeKeys * tile;
             const size_t row0 = (size_t)__shfl_sync(0xffffffffu, pages, tile & 31) * page_stride +
                                 (size_t)(pos & page_mask) * head;
@@ -607,8 +611,9 @@ cudaError_t launch_pages_decode(const PagesView &p, int layer, const StepSeq *se
         int n = 0;
         const cudaError_t e = decode_ready<NB, F32>(&n);
         if (e != cudaSuccess) return e;
-        k_pages_decode<NB, F32><<<grid, 32 * kDecodeWarps, kDecodeWarps * Ring<NB, F32>::Bytes, s>>>(
-            p, layer, seqs, items, scratch, q, out);
+        const cudaError_t l = launch_after(k_pages_decode<NB, F32>, grid, 32 * kDecodeWarps,
+                                           kDecodeWarps * Ring<NB, F32>::Bytes, s, p, layer, seqs, items, scratch, q, out);
+        if (l != cudaSuccess) return l;
         return launched();
     });
 }

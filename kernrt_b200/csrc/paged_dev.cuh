@@ -7,6 +7,30 @@
 
 namespace krt {
 
+// A kernel launched by launch_after may start while the kernel before it on the
+// stream still runs, once all its CTAs have called let_next_start (or ended);
+// behind wait_before, everything that kernel and those before it did is there.
+// What lies before wait_before touches only what older work made (a step's
+// descriptors, pieces and tables: pages_write starts after them and is the only
+// kernel that lets the next one start).
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <class... P, class... A>
+cudaError_t launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s, A... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 // The sequence of the step that holds row r: the last with row0 <= r (row0
 // ascends, empty sequences repeat their successor's row0).
 __device__ __forceinline__ int step_seq_of(const StepSeq *seqs, int n, int r) {

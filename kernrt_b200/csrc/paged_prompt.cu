@@ -231,12 +231,6 @@ __device__ __forceinline__ void split_half(F2 a, uint32_t &hi, uint32_t &neg_lo)
         : "r"(hi), "f"(a.x), "f"(a.y));
     neg_lo = pack_half(d);
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-
 // The power of two that brings a magnitude with these bits to [2^13, 2^14), and
 // its inverse (both normal: magnitudes below 2^-112 get 2^126).
 __device__ __forceinline__ float up_scale(uint32_t bits) {
@@ -353,6 +347,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     };
     // (rows ascend, so n0 <= n1 unless there is no second tile)
     const int n0 = tiles_of(0), n1 = tiles_of(1), n = max(n0, n1);
+    wait_before();
     // The order of the work on (key tile i, query tile t): the s-th takes score
     // buffer s % 3.
     //   s = 2 i + t while both tiles have keys, then n0 + i; n1 = 0: s = i
@@ -813,8 +808,9 @@ cudaError_t launch(const PagesView &p, int layer, const StepSeq *seqs, const Att
         if (e != cudaSuccess) return e;
         attr_done[dev] = true;
     }
-    k_pages_prompt<D, F32><<<(unsigned)p.kv_heads * (unsigned)n_items, kPromptThreads, Shape<D, F32>::Smem, s>>>(
-        p, layer, seqs, items, scratch, q, out, err);
+    const cudaError_t e = launch_after(k_pages_prompt<D, F32>, dim3((unsigned)p.kv_heads * (unsigned)n_items),
+                                       kPromptThreads, Shape<D, F32>::Smem, s, p, layer, seqs, items, scratch, q, out, err);
+    if (e != cudaSuccess) return e;
     count_launch();
     return cudaGetLastError();
 }

@@ -207,15 +207,6 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
     const int limit = live ? min(it.hi, sq.ctx + token + 1) : 0;
     const size_t q_at = ((size_t)(sq.row0 + token) * p.heads + (size_t)j * p.group + (m_row - token * p.group)) * head;
 
-    // this warp's tiles: 16 positions at lo + 16 warp, step 64; a tile never
-    // leaves its page
-    const int t0 = it.lo + 16 * warp;
-    const int n_tiles = it.hi > t0 ? (it.hi - t0 + kDecodeKeys - 1) / kDecodeKeys : 0;
-    const auto page_ids = [&](int tile) {  // lane i: the page of tile + i
-        const int at = t0 + kDecodeKeys * (tile + lane);
-        return at < it.hi ? __ldg(table + (at >> p.page_shift)) : 0;
-    };
-    int pages = page_ids(0);  // of the current 32 tiles
     wait_before();
 
     QFrag<NB> qf;
@@ -262,14 +253,22 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
         m_out = m;
     };
 
+    // this warp's tiles: 16 positions at lo + 16 warp, step 64; a tile never
+    // leaves its page
+    const int t0 = it.lo + 16 * warp;
+    const int n_tiles = it.hi > t0 ? (it.hi - t0 + kDecodeKeys - 1) / kDecodeKeys : 0;
     unsigned char *const mine = ring + warp * G::Bytes;
     const uint32_t mine_at = (uint32_t)__cvta_generic_to_shared(mine);
+    int pages = 0;  // lane i: the page of tile i of the current 32
     const char *const kv = static_cast<const char *>(p.kv);
     constexpr int Size = F32 ? 4 : 2, PerRow = G::Row / 16;  // chunks of a row in shared memory
     const int have = head * Size / 16;                       // of them in a page
     const auto fetch = [&](int tile) {
         if (tile < n_tiles) {
-            if ((tile & 31) == 0 && tile > 0) pages = page_ids(tile);
+            if ((tile & 31) == 0) {
+                const int at = t0 + kDecodeKeys * (tile + lane);
+                pages = at < it.hi ? __ldg(table + (at >> p.page_shift)) : 0;
+            }
             const int pos = t0 + kDecodeKeys * tile;
             const size_t row0 = (size_t)__shfl_sync(0xffffffffu, pages, tile & 31) * page_stride +
                                 (size_t)(pos & page_mask) * head;

@@ -99,6 +99,11 @@ static __device__ __noinline__ RowAcc attend_row(const PagesView &p, int layer, 
         a.l = __fmaf_rn(a.l, keep, sum);
 #pragma unroll
         for (int i = 0; i < kHeadMax / 32; ++i) a.o[i] *= keep;
+        if (a.l != a.l) {  // a NaN score: the whole row is NaN
+#pragma unroll
+            for (int i = 0; i < kHeadMax / 32; ++i) a.o[i] = a.l;
+            break;
+        }
         const int n = min(32, hi - t0);
         for (int s = 0; s < n; ++s) {
             const float ws = __shfl_sync(0xffffffffu, w, s);

@@ -17,11 +17,13 @@
 // tile's largest, f32 values (as two halves, three products) to 2^-22 of their
 // own and 2^-38 of the tile's largest; query rows likewise, row by row.
 // The scales return as one factor of the scores and one of the tile's sum.
-// Where a tile's magnitudes spread so far that some eight neighbouring elements
-// lie 2^18 below its largest (or it holds an infinity or NaN), the CTA's rows are
-// attended again by attend_row in f32, each over the keys it sees alone; so are
-// rows whose result is not finite.  What stands in masked places (later
-// positions of the same prompt included) therefore never reaches a row.
+// Where a tile's magnitudes spread so far that some group of neighbouring
+// elements (four of bf16, eight of f32) lies 2^18 below its largest, or it holds
+// an infinity, the CTA's rows are attended again by attend_row in f32, each over
+// the keys it sees alone; so are rows whose result is not finite, unless their sum
+// of weights is NaN: that takes a NaN score the row does see, and the row is NaN.
+// What stands in masked places (later positions of the same prompt included)
+// therefore never reaches a row.  (NaN stays out of the tiles' largest.)
 // The tensor cores add into an f32 accumulator with truncation: measured
 // relative error 1.1e-9 per K (9e-6 at K = 8192, always toward zero), so
 // a tile's sum of V is taken out of TMEM after every 64 or 128 keys and added in
@@ -245,6 +247,13 @@ __device__ __forceinline__ bool too_wide(uint32_t most, uint32_t least_1) {
     return most >= 0x7f800000u || (most != 0 && (int)(most >> 23) - (int)((least_1 + 1) >> 23) > 18);
 }
 
+// The bits of the largest magnitude of eight f32 (NaN left out).
+__device__ __forceinline__ uint32_t most_of(const float4 &a, const float4 &b) {
+    const float x = fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w)));
+    const float y = fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w)));
+    return __float_as_uint(fmaxf(fmaxf(x, y), 0.0f));
+}
+
 // Byte offset of 16-byte chunk c of row r in a 128-byte swizzled sub-tile.
 __device__ __forceinline__ uint32_t swizzled(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 
@@ -266,9 +275,10 @@ __device__ __forceinline__ uint32_t to_half(uint32_t u, __nv_bfloat162 s) {
     u = *reinterpret_cast<const uint32_t *>(&v);
     return pack_half(pair(u << 16, u & 0xffff0000u));
 }
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+// (max.bf16x2 leaves NaN out: the larger of the others)
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
     uint32_t d;
-    asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
 __device__ __forceinline__ uint32_t min_u16x2(uint32_t a, uint32_t b) {
@@ -387,10 +397,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) {
                 const float4 a = x[2 * c], b = x[2 * c + 1];
-                const uint32_t m = max(max(max(__float_as_uint(fabsf(a.x)), __float_as_uint(fabsf(a.y))),
-                                           max(__float_as_uint(fabsf(a.z)), __float_as_uint(fabsf(a.w)))),
-                                       max(max(__float_as_uint(fabsf(b.x)), __float_as_uint(fabsf(b.y))),
-                                           max(__float_as_uint(fabsf(b.z)), __float_as_uint(fabsf(b.w)))));
+                const uint32_t m = most_of(a, b);
                 most = max(most, m);
                 least = min(least, m - 1);
             }
@@ -508,9 +515,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
         if (S::Sums == 2 && ok && mine) ok = flush(mine - 1);
         if (ok) {
-            bool fine = isfinite(l) && !*(volatile int *)&s_wild;
+            bool fine = isfinite(l);
 #pragma unroll
             for (int d = 0; d < D / 2; ++d) fine = fine && isfinite(acc[d].x) && isfinite(acc[d].y);
+            fine = fine || l != l;  // (a NaN score among the row's own: dividing by l says so)
+            fine = fine && !*(volatile int *)&s_wild;
             const size_t part = ((size_t)item * p.kv_heads + j) * kRows + r;
             if (live && fine) {
                 const float f = it.n_parts == 1 ? 1.0f / l : 0x1p-14f;
@@ -589,11 +598,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             if constexpr (F32) {
 #pragma unroll
                 for (int k = 0; k < Loads; ++k) {
-                    const uint32_t a = max(max(v[2 * k].x & 0x7fffffffu, v[2 * k].y & 0x7fffffffu),
-                                           max(v[2 * k].z & 0x7fffffffu, v[2 * k].w & 0x7fffffffu));
-                    const uint32_t b = max(max(v[2 * k + 1].x & 0x7fffffffu, v[2 * k + 1].y & 0x7fffffffu),
-                                           max(v[2 * k + 1].z & 0x7fffffffu, v[2 * k + 1].w & 0x7fffffffu));
-                    const uint32_t m = max(a, b);
+                    const uint32_t m = most_of(*reinterpret_cast<const float4 *>(&v[2 * k]),
+                                               *reinterpret_cast<const float4 *>(&v[2 * k + 1]));
                     most = max(most, m);
                     least = min(least, m - 1);
                 }
@@ -601,9 +607,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 uint32_t hi = 0, lo = 0xffffffffu;
 #pragma unroll
                 for (int k = 0; k < Loads; ++k) {
-                    const uint32_t m = max_u16x2(max_u16x2(v[k].x & 0x7fff7fffu, v[k].y & 0x7fff7fffu),
-                                                 max_u16x2(v[k].z & 0x7fff7fffu, v[k].w & 0x7fff7fffu));
-                    hi = max_u16x2(hi, m);
+                    const uint32_t m = max_bf16x2(max_bf16x2(v[k].x & 0x7fff7fffu, v[k].y & 0x7fff7fffu),
+                                                  max_bf16x2(v[k].z & 0x7fff7fffu, v[k].w & 0x7fff7fffu));
+                    hi = max_bf16x2(hi, m);
                     lo = min_u16x2(lo, __vsub2(m, 0x00010001u));
                 }
                 most = max(hi << 16, hi & 0xffff0000u);

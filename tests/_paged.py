@@ -4,16 +4,20 @@
 the cache's kind holds them) in 64 bits; `attend` is the definition of the
 attention over them, with the bound its result is held to.
 
-The bound, per output element, from the arithmetic: queries and (f32) keys are
-taken as two bf16 halves (each rounding is off by at most 2^-9, so the second
-half's by 2^-18 of the value; the product of both halves' second parts is at
-most another 2^-18), so a score is off by at most 3 * 2^-18 sum |q k| / sqrt(D)
-and, summed in f32 over D terms (tensor cores truncate: 2^-23 a term), D 2^-23 of
-the same sum more; dx is its largest over the row's keys.  exp(x) is then off by
-the factor exp(dx), and again in the sum of the weights; 2^-17 covers
-the exponential itself and the running rescale.  Weights (and f32 values) split
-into halves cost 3 * 2^-18, and the sums over n keys, in steps of 16, (n / 16 +
-16) 2^-23.  All act on sum p |v|.
+The bound, per output element, from the arithmetic.  Queries, weights and (f32)
+keys and values are taken as two fp16 halves after a scaling by powers of two
+(each rounding is off by at most 2^-11 of what it rounds, the second half's by
+2^-22 of the value, and so is the product of two second halves that is left
+out) or as three bf16 parts (better still), so a score is off by at most
+3 * 2^-22 sum |q k| / sqrt(D) and, summed in f32 over D terms (tensor cores truncate:
+2^-23 a term), by D 2^-23 of the same sum more; dx is its largest over the row's
+keys.  A weight exp(x - max) is then off by the factor exp(dx), and so is the sum of
+the weights; its argument is rounded in powers of two, by at most 2^-23 |x - max| /
+ln 2, which times the weight is at most 2^-23; 2^-18 covers that, the exponential
+(2^-22) and the rescales of a few hundred tiles' running maximum (2^-23 each,
+only where the maximum grows).  Halves of weights and values cost 3 * 2^-22, the
+tensor cores' sums over a tile of at most 256 keys in steps of 16 32 * 2^-23, and
+n / 64 + 16 additions of tiles and pieces 2^-24 each.  All act on sum p |v|.
 """
 import math
 
@@ -31,24 +35,25 @@ def rounded(x, kind):
     return t.double().numpy()
 
 
-def attend(q, keys, vals, group, first):
+def attend(q, keys, vals, group, first, heads=None):
     """q [n, H, D] in 64 bits, keys and vals [L, HK, D]; row i sees keys 0 .. first + i.
-    Returns out [n, H, D] and its bound."""
-    n, heads, d = q.shape
-    out, bound = np.empty((n, heads, d)), np.empty((n, heads, d))
+    Returns out [n, H, D] and its bound (of some heads, if given)."""
+    n, all_heads, d = q.shape
+    heads = range(all_heads) if heads is None else heads
+    out, bound = np.empty((n, len(heads), d)), np.empty((n, len(heads), d))
     with np.errstate(all="ignore"):
         for i in range(n):
             m = first + i + 1
             k, v = keys[:m], vals[:m]
-            for h in range(heads):
+            for z, h in enumerate(heads):
                 kj, vj = k[:, h // group], v[:, h // group]
                 x = kj @ q[i, h] / math.sqrt(d)
-                dx = float((np.abs(kj) @ np.abs(q[i, h])).max()) / math.sqrt(d) * (3 * 2.0 ** -18 + d * 2.0 ** -23)
+                dx = float((np.abs(kj) @ np.abs(q[i, h])).max()) / math.sqrt(d) * (3 * 2.0 ** -22 + d * 2.0 ** -23)
                 p = np.exp(x - x.max())
                 p /= p.sum()
-                out[i, h] = p @ vj
-                rel = 2 * math.expm1(min(dx, 50.0)) + 2.0 ** -17 + 3 * 2.0 ** -18 + (m / 16 + 16) * 2.0 ** -23
-                bound[i, h] = rel * (p @ np.abs(vj))
+                out[i, z] = p @ vj
+                rel = 2 * math.expm1(min(dx, 50.0)) + 2.0 ** -18 + 3 * 2.0 ** -22 + 32 * 2.0 ** -23 + (m / 64 + 16) * 2.0 ** -24
+                bound[i, z] = rel * (p @ np.abs(vj))
     return out, bound
 
 
@@ -106,7 +111,7 @@ class Pair:
         return [(scale * rng.standard_normal((n, w))).astype(np.float32)
                 for w in (self.heads * self.head, self.kv_heads * self.head, self.kv_heads * self.head)]
 
-    def step(self, seqs, rows, data, check=True, check_rows=None):
+    def step(self, seqs, rows, data, check=True, check_rows=None, heads=None):
         """One step over all layers; data[layer] = (q, k, v).  Returns the outputs."""
         b = self.b
         b.pages_step(self.p, seqs, rows)
@@ -135,8 +140,9 @@ class Pair:
                     keys, vals = (np.stack(x) for x in self.kv[s][layer])
                     q64 = q[at:at + n].astype(np.float64).reshape(n, self.heads, self.head)
                     for i in some:
-                        want, bound = attend(q64[i:i + 1], keys, vals, self.heads // self.kv_heads, first + i)
-                        same(outs[layer][at + i], want[0], bound[0], f"layer {layer} sequence {s} row {i} of {n}, "
+                        want, bound = attend(q64[i:i + 1], keys, vals, self.heads // self.kv_heads, first + i, heads)
+                        got = outs[layer][at + i]
+                        same(got if heads is None else got[heads], want[0], bound[0], f"layer {layer} sequence {s} row {i} of {n}, "
                                                                      f"{first} before")
                 at += n
         return outs

@@ -157,7 +157,7 @@ SIGNATURES = {
     "kernrt_cuda_seq_copy": (C.c_int, [P, C.c_uint64, C.c_uint64, SZ, C.POINTER(C.c_uint64)]),
     "kernrt_cuda_seq_trim": (C.c_int, [P, C.c_uint64, C.c_uint64, SZ]),
     "kernrt_cuda_seq_close": (C.c_int, [P, C.c_uint64, P, SZ]),
-    "kernrt_cuda_seq_table": (C.c_int, [P, C.c_uint64, C.c_uint64, C.POINTER(SZ), P, SZ, C.POINTER(SZ)]),
+    "kernrt_cuda_seq_table": (C.c_int, [P, C.c_uint64, C.c_uint64, P, P, SZ, P]),
     "kernrt_cuda_pages_compact": (C.c_int, [P, C.c_uint64, C.POINTER(SZ)]),
     "kernrt_cuda_pages_step": (C.c_int, [P, C.c_uint64, P, P, SZ]),
     "kernrt_cuda_pages_write": (C.c_int, [P, C.c_uint64, SZ, Buf, Buf]),
@@ -234,8 +234,7 @@ class CudaBackend:
         _ok(self._lib.kernrt_cuda_create(int(device), C.byref(ctx)))
         self._ctx = ctx
         self._lens: dict[int, int] = {}
-        room = np.empty(1024, np.int32)
-        self._room = (room, _ptr(room), (SZ * 1)())  # where seq_table reads to
+        self._make_room(1024)
 
     # -- lifecycle ----------------------------------------------------------------
     def close(self) -> None:
@@ -532,13 +531,17 @@ class CudaBackend:
 
     def seq_table(self, pages: int, seq: int) -> np.ndarray:
         """The ids of the sequence's pages (int32)."""
-        room, at, n = self._room
-        _ok(self._lib.kernrt_cuda_seq_table(self._ctx, pages, seq, None, at, room.size, n))
-        if n[0] > room.size:
-            room = np.empty(2 * n[0], np.int32)
-            self._room = (room, _ptr(room), n)
+        room, at, size, count, n = self._room
+        _ok(self._lib.kernrt_cuda_seq_table(self._ctx, pages, seq, None, at, size, n))
+        if count.value > size:
+            self._make_room(2 * count.value)
             return self.seq_table(pages, seq)
-        return room[:n[0]].copy()
+        return room[:count.value].copy()
+
+    def _make_room(self, size: int) -> None:
+        """Where seq_table reads to."""
+        room, count = np.empty(size, np.int32), SZ()
+        self._room = (room, _ptr(room), size, count, C.addressof(count))
 
     def pages_compact(self, pages: int) -> int:
         """Moves the pages in use to the front of the pool; returns how many moved."""

@@ -1736,12 +1736,10 @@ public:
             if (b) std::memcpy(block.data() + a, delta.data(), b);
             if (!copies.empty()) std::memcpy(block.data() + a + b, copies.data(), copies.size() * sizeof(CopyItem));
             const char *d = static_cast<const char *>(stage(block.data(), block.size()));
-            launch_or_fail(launch_pages_step(reinterpret_cast<const StepSeq *>(d), (int)desc.size(), c.seqs, c.table,
-                                             c.view.max_pages, stream_),
+            launch_or_fail(launch_pages_step(c.view, reinterpret_cast<const StepSeq *>(d), (int)desc.size(), c.seqs,
+                                             c.table, reinterpret_cast<const CopyItem *>(d + a + b),
+                                             (int)copies.size(), stream_),
                            "pages_step");
-            launch_or_fail(launch_pages_copy(c.view, reinterpret_cast<const CopyItem *>(d + a + b), (int)copies.size(),
-                                             stream_),
-                           "pages_step (copies)");
             for (const StepSeq &q : desc) c.map->at((size_t)q.slot).dirty = c.map->at((size_t)q.slot).pages.size();
         }
         c.step = std::move(desc);

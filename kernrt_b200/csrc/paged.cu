@@ -15,16 +15,6 @@ cudaError_t launched() {
     return cudaGetLastError();
 }
 
-// One CTA per sequence: its descriptor, and the table entries that changed.
-__global__ void __launch_bounds__(128) k_pages_step(const StepSeq *__restrict__ staged, StepSeq *__restrict__ seqs,
-                                                    int32_t *__restrict__ table, int max_pages) {
-    const StepSeq q = staged[blockIdx.x];
-    const int32_t *delta = reinterpret_cast<const int32_t *>(staged + gridDim.x) + q.delta;
-    if (threadIdx.x == 0) seqs[blockIdx.x] = q;
-    for (int i = threadIdx.x; i < q.n_dirty; i += blockDim.x)
-        table[(size_t)q.slot * max_pages + q.dirty + i] = delta[i];
-}
-
 // Eight elements of a k or v row per thread; the row's page comes from the
 // sequence's table.
 __global__ void __launch_bounds__(256) k_pages_write(PagesView p, int layer, const StepSeq *__restrict__ seqs, int n,
@@ -60,17 +50,20 @@ __global__ void __launch_bounds__(256) k_pages_write(PagesView p, int layer, con
 // One warp per 4 KB of (copy, layer, K or V, kv head), whose used rows are
 // contiguous in a page: eight loads in flight a lane, and pieces small enough
 // that the last wave is short (measured, 33 pages of 64 x 128 f32, 8 heads, 24
-// layers, 830 MB moved: a warp per whole head and page 163 us, 4 KB pieces below).
+// layers, 830 MB moved: a warp per whole head and page 163 us, 4 KB pieces 138).
 constexpr int kCopyChunks = 256;  // of 16 bytes
-__global__ void __launch_bounds__(256) k_pages_copy(PagesView p, const CopyItem *__restrict__ items, int pieces,
-                                                    size_t units) {
+struct Copies {
+    const CopyItem *items;
+    int pieces;    // of a head's part of a page
+    size_t units;  // pieces in all
+};
+__device__ __forceinline__ void copy_piece(const PagesView &p, const Copies &copies, size_t u) {
+    if (u >= copies.units) return;
     const int lane = threadIdx.x & 31;
-    const size_t u = blockIdx.x * (size_t)(blockDim.x / 32) + (threadIdx.x >> 5);
-    if (u >= units) return;
     const size_t size = p.f32 ? 4 : 2;
-    const size_t head_unit = u / pieces;
-    const int per_copy = p.n_layers * 2 * p.kv_heads, first = (int)(u - head_unit * pieces) * kCopyChunks;
-    const CopyItem c = items[head_unit / per_copy];
+    const size_t head_unit = u / copies.pieces;
+    const int per_copy = p.n_layers * 2 * p.kv_heads, first = (int)(u - head_unit * copies.pieces) * kCopyChunks;
+    const CopyItem c = copies.items[head_unit / per_copy];
     const int rest = (int)(head_unit % per_copy), j = rest % p.kv_heads, lk = rest / p.kv_heads;
     const int n = (int)((size_t)c.rows * p.head * size / 16) - first;
     const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const char *>(p.kv) +
@@ -85,6 +78,34 @@ __global__ void __launch_bounds__(256) k_pages_copy(PagesView p, const CopyItem 
 #pragma unroll
     for (int i = 0; i < kCopyChunks / 32; ++i)
         if (lane + 32 * i < n) dst[lane + 32 * i] = v[i];
+}
+
+__global__ void __launch_bounds__(256) k_pages_copy(PagesView p, Copies copies) {
+    copy_piece(p, copies, blockIdx.x * (size_t)8 + (threadIdx.x >> 5));
+}
+
+Copies copies_of(const PagesView &p, const CopyItem *items, int n) {
+    Copies c{items, 0, 0};
+    const int chunks = (int)(((size_t)p.head << p.page_shift) * (p.f32 ? 4 : 2) / 16);
+    c.pieces = (chunks + kCopyChunks - 1) / kCopyChunks;
+    c.units = (size_t)n * p.n_layers * 2 * p.kv_heads * c.pieces;
+    return c;
+}
+
+// A step's first n CTAs bring a sequence's descriptor and the table entries
+// that changed; the others copy the shared pages that sequences grow into.
+__global__ void __launch_bounds__(256) k_pages_step(PagesView p, const StepSeq *__restrict__ staged, int n,
+                                                    StepSeq *__restrict__ seqs, int32_t *__restrict__ table,
+                                                    Copies copies) {
+    if (blockIdx.x >= (unsigned)n) {
+        copy_piece(p, copies, (blockIdx.x - (unsigned)n) * (size_t)8 + (threadIdx.x >> 5));
+        return;
+    }
+    const StepSeq q = staged[blockIdx.x];
+    const int32_t *delta = reinterpret_cast<const int32_t *>(staged + n) + q.delta;
+    if (threadIdx.x == 0) seqs[blockIdx.x] = q;
+    for (int i = threadIdx.x; i < q.n_dirty; i += blockDim.x)
+        table[(size_t)q.slot * p.max_pages + q.dirty + i] = delta[i];
 }
 
 // ---- single tokens: attention split over the length ------------------------------
@@ -107,7 +128,8 @@ __global__ void __launch_bounds__(256) k_pages_copy(PagesView p, const CopyItem 
 // accumulator of part 1; a thread then finds the parts of one score in its own
 // registers.  An f32 cache is split the same way, and the products down to
 // 2^-24 are kept: (x1 + x2) k1, x3 k1, (x1 + x2) k2, x1 k3.  The MMAs add with
-// truncation, so after every 16 tiles the sums go to shared memory, where they
+// truncation, so the small products are summed apart from the large ones, and
+// after every 16 tiles the sums go to shared memory, where they
 // are added with rounding (added in registers after every tile, 64 x 8000 keys of
 // 16 heads of 128 took 207 us instead of 177).
 template <int NB>
@@ -187,6 +209,11 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
                    AttnScratch scratch, const float *__restrict__ q, float *__restrict__ out) {
     constexpr int NV = (NB + 1) / 2;  // blocks of 64 of the values
     constexpr int R = kDecodeRows;
+    // f32 heads of more than 64 have no registers to sum their small products
+    // apart, and put their sums out more often instead (131,072 x 8 heads of 128:
+    // 217 us, spilling for it 239)
+    constexpr bool kApart = NB <= 2;
+    constexpr int kRun = F32 && !kApart ? 4 : 16;  // tiles between put_out
     using G = Ring<NB, F32>;
     extern __shared__ __align__(128) unsigned char ring[];
     __shared__ float s_o[kDecodeWarps][R][32 * NB + 4];
@@ -297,7 +324,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
         float s[2][2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            // the products of the first parts, and all the smaller ones
+            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f}, e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             const int key = 8 * u + 4 * (g & 1) + (g >> 1);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -311,9 +339,9 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
                         split3(kc.v[h].z, kc.v[h].w, k1[1], k2[1], k3[1]);
                         const uint32_t(&a)[4] = qf.a[b][h];
                         mma16816(c, a[0], a[1], a[2], a[3], k1[0], k1[1]);
-                        mma16816(c, a[0], a[1], a[2], a[3], k2[0], k2[1]);
-                        mma16816(c, a[0], 0, a[2], 0, k3[0], k3[1]);
-                        mma16816(c, qf.c[b][h][0], 0, qf.c[b][h][1], 0, k1[0], k1[1]);
+                        mma16816(e, a[0], a[1], a[2], a[3], k2[0], k2[1]);
+                        mma16816(e, a[0], 0, a[2], 0, k3[0], k3[1]);
+                        mma16816(e, qf.c[b][h][0], 0, qf.c[b][h][1], 0, k1[0], k1[1]);
                     }
                 } else {
                     const uint32_t k[4] = {kc.v.x, kc.v.y, kc.v.z, kc.v.w};
@@ -321,15 +349,15 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
                     for (int h = 0; h < 2; ++h) {
                         const uint32_t(&a)[4] = qf.a[b][h];
                         mma16816(c, a[0], a[1], a[2], a[3], k[2 * h], k[2 * h + 1]);
-                        mma16816(c, qf.c[b][h][0], 0, qf.c[b][h][1], 0, k[2 * h], k[2 * h + 1]);
+                        mma16816(e, qf.c[b][h][0], 0, qf.c[b][h][1], 0, k[2 * h], k[2 * h + 1]);
                     }
                 }
             }
-            // rows 0-7 hold parts 1 and 3, rows 8-15 part 2 of the same score;
+            // rows 0-7 hold part 1 (and 3), rows 8-15 part 2 of the same score;
             // columns 2 t and 2 t + 1 are keys 8 u + t and 8 u + 4 + t
             const int at = pos + 8 * u + t;
-            s[u][0] = at < limit ? (c[0] + c[2]) * scale : -INFINITY;
-            s[u][1] = at + 4 < limit ? (c[1] + c[3]) * scale : -INFINITY;
+            s[u][0] = at < limit ? (c[0] + (c[2] + (e[0] + e[2]))) * scale : -INFINITY;
+            s[u][1] = at + 4 < limit ? (c[1] + (c[3] + (e[1] + e[3]))) * scale : -INFINITY;
         }
         float mt = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
@@ -376,10 +404,15 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
                     uint32_t v1[2], v2[2], v3[2];
                     split3(e[0], e[1], v1[0], v2[0], v3[0]);
                     split3(e[2], e[3], v1[1], v2[1], v3[1]);
+                    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float(&small)[4] = kApart ? c : o[b][i];
+                    mma16816(small, pa[0], pa[1], pa[2], pa[3], v2[0], v2[1]);
+                    mma16816(small, pa[0], 0, pa[2], 0, v3[0], v3[1]);
+                    mma16816(small, pc[0], 0, pc[1], 0, v1[0], v1[1]);
                     mma16816(o[b][i], pa[0], pa[1], pa[2], pa[3], v1[0], v1[1]);
-                    mma16816(o[b][i], pa[0], pa[1], pa[2], pa[3], v2[0], v2[1]);
-                    mma16816(o[b][i], pa[0], 0, pa[2], 0, v3[0], v3[1]);
-                    mma16816(o[b][i], pc[0], 0, pc[1], 0, v1[0], v1[1]);
+                    if (kApart)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) o[b][i][x] += c[x];
                 }
             } else {
 #pragma unroll
@@ -392,7 +425,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
                 }
             }
         }
-        if ((tile & 15) == 15) put_out();
+        if (tile % kRun == kRun - 1) put_out();
     }
 
     // the CTA's warps meet in shared memory
@@ -528,10 +561,13 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
 
 }  // namespace
 
-cudaError_t launch_pages_step(const StepSeq *staged, int n, StepSeq *seqs, int32_t *table, int max_pages,
-                              cudaStream_t s) {
+cudaError_t launch_pages_step(const PagesView &p, const StepSeq *staged, int n, StepSeq *seqs, int32_t *table,
+                              const CopyItem *items, int n_items, cudaStream_t s) {
     if (n == 0) return cudaSuccess;
-    k_pages_step<<<(unsigned)n, 128, 0, s>>>(staged, seqs, table, max_pages);
+    const Copies c = copies_of(p, items, n_items);
+    const size_t grid = (size_t)n + (c.units + 7) / 8;
+    if (grid > (size_t)INT32_MAX) return cudaErrorInvalidValue;
+    k_pages_step<<<(unsigned)grid, 256, 0, s>>>(p, staged, n, seqs, table, c);
     return launched();
 }
 
@@ -547,11 +583,9 @@ cudaError_t launch_pages_write(const PagesView &p, int layer, const StepSeq *seq
 
 cudaError_t launch_pages_copy(const PagesView &p, const CopyItem *items, int n, cudaStream_t s) {
     if (n == 0) return cudaSuccess;
-    const int chunks = (int)(((size_t)p.head << p.page_shift) * (p.f32 ? 4 : 2) / 16);
-    const int pieces = (chunks + kCopyChunks - 1) / kCopyChunks;
-    const size_t units = (size_t)n * p.n_layers * 2 * p.kv_heads * pieces;
-    if ((units + 7) / 8 > (size_t)INT32_MAX) return cudaErrorInvalidValue;
-    k_pages_copy<<<(unsigned)((units + 7) / 8), 256, 0, s>>>(p, items, pieces, units);
+    const Copies c = copies_of(p, items, n);
+    if ((c.units + 7) / 8 > (size_t)INT32_MAX) return cudaErrorInvalidValue;
+    k_pages_copy<<<(unsigned)((c.units + 7) / 8), 256, 0, s>>>(p, c);
     return launched();
 }
 

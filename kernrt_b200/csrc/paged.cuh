@@ -50,10 +50,10 @@ struct CopyItem {
     int32_t src, dst, rows;
 };
 
-// staged: StepSeq[n], then the table deltas; copies the descriptors to `seqs`
-// and the deltas into the table.
-cudaError_t launch_pages_step(const StepSeq *staged, int n, StepSeq *seqs, int32_t *table, int max_pages,
-                              cudaStream_t s);
+// staged: StepSeq[n], then the table deltas; copies the descriptors to `seqs`,
+// the deltas into the table, and the pages of `items`.
+cudaError_t launch_pages_step(const PagesView &p, const StepSeq *staged, int n, StepSeq *seqs, int32_t *table,
+                              const CopyItem *items, int n_items, cudaStream_t s);
 // Row r of k and v [rows, kv_heads * head] f32 into its position of `layer`.
 cudaError_t launch_pages_write(const PagesView &p, int layer, const StepSeq *seqs, int n, int rows, const float *k,
                                const float *v, cudaStream_t s);

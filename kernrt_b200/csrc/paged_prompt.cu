@@ -27,7 +27,8 @@
 // The tensor cores add into an f32 accumulator with truncation: measured
 // relative error 1.1e-9 per K (9e-6 at K = 8192, always toward zero), so
 // a tile's sum of V is taken out of TMEM after every 64 or 128 keys and added in
-// registers with rounding.
+// registers with rounding, and the products of the second halves, small ones, come
+// first.
 //
 // One CTA: 256 query rows as two M = 128 tiles, so that the softmax of one runs
 // under the MMAs of the other.  Warps 0-3 and 4-7: a thread per row of the two
@@ -672,13 +673,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 const uint32_t a = here(k_desc(base + t * S::QTile)), k = here(k_desc(slots + slot * S::Slot));
                 const uint32_t d_at = here(tmem + buf * Keys);
 #pragma unroll 1
-                for (int x = 0; x < S::Parts + 1; ++x) {  // q_hi K_hi, q_lo K_hi, q_hi K_lo
+                for (int y = 0; y < S::Parts + 1; ++y) {  // q_lo K_hi, q_hi K_lo, q_hi K_hi
+                    const int x = y < S::Parts ? y + 1 : 0;
                     const int qo = x == 1 ? (D / 64) * 16384 : 0, ko = x == 2 ? (D / 64) * S::Sub : 0;
 #pragma unroll
                     for (int d = 0; d < D / 16; ++d)
                         mma_ss(d_at, a + ((qo + (d >> 2) * 16384 + (d & 3) * 32) >> 4),
                                k + ((ko + (d >> 2) * S::Sub + (d & 3) * 32) >> 4), idesc<Keys, false>(x == 1, x == 2),
-                               x | d);
+                               y | d);
                 }
             };
             const auto values = [&](auto t, int slot, int buf) {  // O = (w_hi + w_lo) V
@@ -686,12 +688,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 const uint32_t v = here(mn_desc(slots + slot * S::Slot, S::Sub)), w = here(tmem + buf * Keys);
                 const uint32_t d_at = here(tmem + S::SumAt + (S::Sums == 2 ? t * D : 0));
 #pragma unroll 1
-                for (int x = 0; x < S::Parts + 1; ++x) {  // w_hi V_hi, w_lo V_hi, w_hi V_lo
+                for (int y = 0; y < S::Parts + 1; ++y) {  // w_lo V_hi, w_hi V_lo, w_hi V_hi
+                    const int x = y < S::Parts ? y + 1 : 0;
                     const int vo = x == 2 ? (D / 64) * S::Sub : 0;
 #pragma unroll
                     for (int k = 0; k < Keys / 16; ++k)
                         mma_ts(d_at, w + k * 16 / W * W + k * 16 % W / 2 + (x == 1 ? W / 2 : 0), v + ((vo + k * 2048) >> 4),
-                               idesc<D, true>(x == 1, x == 2), x | k);
+                               idesc<D, true>(x == 1, x == 2), y | k);
                 }
             };
             const auto commit = [&](uint64_t *bar) {

@@ -1701,7 +1701,7 @@ public:
             if (rows[i] > (uint64_t)INT32_MAX) fail(KERNRT_E_INVALID, "too many rows in one step");
             total += (size_t)rows[i];
         }
-        fits_int(total * 2, "pages_step");
+        fits_int(total * (size_t)std::max(2, c.view.group), "pages_step");
         flush();
         std::vector<PageCopy> copies;
         paging([&] { c.map->extend(seqs, rows, n, &copies); });

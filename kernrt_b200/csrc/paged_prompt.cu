@@ -13,17 +13,21 @@
 // bf16 three), which doubles the MMA work instead of tripling it.  Both operands
 // of an MMA are then fp16, so the CTA's loader turns page rows into fp16: every
 // tile of K or V is multiplied by the power of two that brings its largest
-// magnitude to [2^13, 2^14), which keeps bf16 values exact down to 2^-28 of the
-// tile's largest, f32 values (as two halves, three products) to 2^-22 of their
-// own and 2^-38 of the tile's largest; query rows likewise, row by row.
-// The scales return as one factor of the scores and one of the tile's sum.
-// Where a tile's magnitudes spread so far that some group of neighbouring
-// elements (four of bf16, eight of f32) lies 2^18 below its largest, or it holds
-// an infinity, the CTA's rows are attended again by attend_row in f32, each over
-// the keys it sees alone; so are rows whose result is not finite, unless their sum
-// of weights is NaN: that takes a NaN score the row does see, and the row is NaN.
-// What stands in masked places (later positions of the same prompt included)
-// therefore never reaches a row.  (NaN stays out of the tiles' largest.)
+// magnitude to [2^13, 2^14), which keeps bf16 values exact down to 2^-31 of the
+// tile's largest, and f32 values (as two halves, three products) to 2^-22 of
+// their own or 2^-39 of the tile's largest, whichever is more; query rows
+// likewise, row by row.  The scales return as one factor of the scores and one of
+// the tile's sum.  A score only needs its absolute error small, and 2^-39 of the
+// largest query and key is far below the rounding of f32 sums.  Values are asked
+// for more, because the tile's largest may stand in a row that is masked or has
+// no weight: where some group of neighbouring values (four of bf16, eight of
+// f32) lies 2^28 (f32: 2^20) below the tile's largest, and above 2^-60 all the
+// same, the CTA's rows are attended again by attend_row in f32, each over the
+// keys it sees alone.  So they are where a tile or a query holds an infinity, and
+// so are rows whose result is not finite, unless their sum of weights is NaN: that
+// takes a NaN score the row does see, and the row is NaN.  What stands in masked
+// places (later positions of the same prompt included) therefore never reaches a
+// row.  (NaN stays out of the tiles' largest.)
 // The tensor cores add into an f32 accumulator with truncation: measured
 // relative error 1.1e-9 per K (9e-6 at K = 8192, always toward zero), so
 // a tile's sum of V is taken out of TMEM after every 64 or 128 keys and added in
@@ -242,10 +246,13 @@ __device__ __forceinline__ float up_scale(uint32_t bits) {
 }
 __device__ __forceinline__ float down_scale(float up) { return __uint_as_float((254u << 23) - __float_as_uint(up)); }
 
-// Whether magnitudes spread too far for one scale (bits of the largest, and of
-// the smallest non-zero largest-of-eight less 1).
-__device__ __forceinline__ bool too_wide(uint32_t most, uint32_t least_1) {
-    return most >= 0x7f800000u || (most != 0 && (int)(most >> 23) - (int)((least_1 + 1) >> 23) > 18);
+// Magnitudes (as f32 bits) less kTiny, unsigned: those below 2^-60, zeros among
+// them, come out above all others.
+constexpr uint32_t kTiny = 67u << 23;
+// Whether values spread too far for one scale: the largest magnitude's bits, and
+// the least of the groups' largest less kTiny.
+__device__ __forceinline__ bool too_wide(uint32_t most, uint32_t least, int bits) {
+    return least < 0x80000000u && (int)(most >> 23) - (int)((least + kTiny) >> 23) > bits;
 }
 
 // The bits of the largest magnitude of eight f32 (NaN left out).
@@ -394,15 +401,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
             for (int c = 0; c < D / 4; ++c)
                 x[c] = live && c < 2 * chunks ? __ldg(src + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            uint32_t most = 0, least = 0xffffffffu;
+            uint32_t most = 0;
 #pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-                const float4 a = x[2 * c], b = x[2 * c + 1];
-                const uint32_t m = most_of(a, b);
-                most = max(most, m);
-                least = min(least, m - 1);
-            }
-            if (too_wide(most, least)) s_wild = 1;
+            for (int c = 0; c < D / 8; ++c) most = max(most, most_of(x[2 * c], x[2 * c + 1]));
+            if (most == 0x7f800000u) s_wild = 1;
             const float up = up_scale(most);
             sc = kLog2e * rsqrtf((float)p.head) * down_scale(up);
             const uint32_t tile = base + (uint32_t)t * S::QTile;
@@ -602,7 +604,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     const uint32_t m = most_of(*reinterpret_cast<const float4 *>(&v[2 * k]),
                                                *reinterpret_cast<const float4 *>(&v[2 * k + 1]));
                     most = max(most, m);
-                    least = min(least, m - 1);
+                    least = min(least, m - kTiny);
                 }
             } else {  // two bf16 a register; the chunks are the four even and the four odd elements
                 uint32_t hi = 0, lo = 0xffffffffu;
@@ -611,11 +613,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     const uint32_t m = max_bf16x2(max_bf16x2(v[k].x & 0x7fff7fffu, v[k].y & 0x7fff7fffu),
                                                   max_bf16x2(v[k].z & 0x7fff7fffu, v[k].w & 0x7fff7fffu));
                     hi = max_bf16x2(hi, m);
-                    lo = min_u16x2(lo, __vsub2(m, 0x00010001u));
+                    lo = min_u16x2(lo, __vsub2(m, kTiny | kTiny >> 16));
                 }
                 most = max(hi << 16, hi & 0xffff0000u);
-                const uint32_t l0 = lo & 0xffffu, l1 = lo >> 16, l = min(l0, l1);
-                least = l == 0xffffu ? 0xffffffffu : ((l + 1) << 16) - 1;
+                least = min(lo << 16, lo & 0xffff0000u);
             }
             most = __reduce_max_sync(0xffffffffu, most);
             least = __reduce_min_sync(0xffffffffu, least);
@@ -633,7 +634,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
             const float up = up_scale(most);
             if (tid == 0) {
-                if (too_wide(most, least)) s_wild = 1;
+                if (most == 0x7f800000u || (is_v(i) && too_wide(most, least, F32 ? 20 : 28))) s_wild = 1;
                 (is_v(i) ? s_vscale : s_kscale)[tile_of(i) & (kScaleRing - 1)] = down_scale(up);
             }
             const uint32_t dst =

@@ -323,6 +323,82 @@ def test_refusals(gpu):
         b.seq_open(c.p)  # destroyed
 
 
+@KINDS
+def test_layer_calls_replay_in_a_graph(gpu, kind):
+    """A step's layer calls captured after its first attention call and replayed
+    on new rows, two graphs over one cache's scratch, a prompt's and a token's
+    pieces in both."""
+    import torch
+
+    from kernrt_b200.interop import as_torch
+
+    rng = np.random.default_rng(81)
+    with Pair(gpu, kind, 16, 8, 128, 32, 300, 4, 4000, layers=2) as c:
+        a, b = c.open(), c.open()
+        c.step([a, b], [1500, 900], [c.rows(rng, 2400) for _ in range(2)], check=False)
+        lens = [700, 1]
+        gpu.pages_step(c.p, [a, b], lens)
+        rows = sum(lens)
+        stream = torch.cuda.ExternalStream(gpu.stream())
+        bufs, graphs = [], []
+        for layer in range(2):
+            hs = [c.up(x) for x in c.rows(rng, rows)] + [c.up(np.zeros((rows, 2048), np.float32))]
+            bufs.append(hs)
+            gpu.pages_write(c.p, layer, hs[1], hs[2])
+            gpu.pages_attention(c.p, layer, hs[0], hs[3])
+        gpu.synchronize()
+        for layer, hs in enumerate(bufs):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                gpu.pages_write(c.p, layer, hs[1], hs[2])
+                gpu.pages_attention(c.p, layer, hs[0], hs[3])
+            graphs.append(g)
+        for _ in range(2):  # new rows through the graphs, then the plain calls
+            want = []
+            for hs in bufs:
+                for h, x in zip(hs, c.rows(rng, rows)):
+                    as_torch(gpu, h, x.shape).copy_(torch.from_numpy(x))
+            torch.cuda.synchronize()
+            for layer, hs in enumerate(bufs):
+                gpu.pages_write(c.p, layer, hs[1], hs[2])
+                gpu.pages_attention(c.p, layer, hs[0], hs[3])
+                want.append(gpu.read(hs[3], rows * 2048))
+                as_torch(gpu, hs[3], (rows * 2048,)).zero_()
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                for g in graphs:
+                    g.replay()
+            torch.cuda.synchronize()
+            for hs, w in zip(bufs, want):
+                assert np.array_equal(gpu.read(hs[3], rows * 2048), w)
+
+
+def test_freed_memory_comes_back_zeroed(gpu):
+    """A freed block serves the next allocation of its size, behind the work that
+    still uses it."""
+    for n in (10, 5000, 3 << 20):
+        h = gpu.upload(np.full(n, 3.0, np.float32))
+        other = gpu.upload(np.full(n, 2.0, np.float32))
+        gpu.add_in_place(other, h, n)
+        gpu.free(h)
+        again = gpu.alloc(n)
+        assert (gpu.read(again, n) == 0).all() and (gpu.read(other, n) == 5).all()
+        gpu.free(again)
+        gpu.free(other)
+    # far more than is kept
+    for _ in range(6):
+        gpu.free(gpu.alloc_bytes(3 << 30))
+    p = gpu.pages_create(BF16, 2, 4, 2, 64, 16, 100, 2, 1000)
+    s = gpu.seq_open(p)
+    gpu.pages_step(p, [s], [100])
+    gpu.pages_destroy(p)
+    q = gpu.pages_create(BF16, 2, 4, 2, 64, 16, 100, 2, 1000)
+    from kernrt_b200.interop import pages_as_torch
+    gpu.synchronize()
+    assert not pages_as_torch(gpu, q).any()
+    gpu.pages_destroy(q)
+
+
 def test_free_waits_for_queued_work_and_ends_the_handle(gpu):
     a = np.arange(1000, dtype=np.float32)
     x, y = gpu.upload(a), gpu.upload(a)

@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import subprocess
+from array import array
 
 import numpy as np
 
@@ -223,6 +224,13 @@ def safetensors_tensor(path: str, name: str) -> dict:
 def _ptr(a: np.ndarray):
     assert a.flags["C_CONTIGUOUS"]
     return a.ctypes.data
+
+
+def _u64(values) -> tuple[array, int, int]:
+    """Handles or counts as 64-bit words: the array that holds them, its address
+    and length (a few words, several times a step: cheaper than through numpy)."""
+    a = array("Q", values.tolist() if isinstance(values, np.ndarray) else values)
+    return (a, *a.buffer_info())
 
 
 class CudaBackend:
@@ -521,8 +529,8 @@ class CudaBackend:
         _ok(self._lib.kernrt_cuda_seq_trim(self._ctx, pages, seq, length))
 
     def seq_close(self, pages: int, seqs) -> None:
-        a = np.ascontiguousarray(seqs, dtype=np.uint64)
-        _ok(self._lib.kernrt_cuda_seq_close(self._ctx, pages, _ptr(a), a.size))
+        a, at, n = _u64(seqs)
+        _ok(self._lib.kernrt_cuda_seq_close(self._ctx, pages, at, n))
 
     def seq_length(self, pages: int, seq: int) -> int:
         n = SZ()
@@ -540,7 +548,7 @@ class CudaBackend:
 
     def _make_room(self, size: int) -> None:
         """Where seq_table reads to."""
-        room, count = np.empty(size, np.int32), SZ()
+        room, count = np.empty(size, np.int32), SZ()  # (kept with their addresses)
         self._room = (room, _ptr(room), size, count, C.addressof(count))
 
     def pages_compact(self, pages: int) -> int:
@@ -551,11 +559,11 @@ class CudaBackend:
 
     def pages_step(self, pages: int, seqs, rows) -> None:
         """Sequence seqs[i] grows by rows[i] positions: the step's rows."""
-        s = np.ascontiguousarray(seqs, dtype=np.uint64)
-        r = np.ascontiguousarray(rows, dtype=np.uint64)
-        if s.shape != r.shape:
+        s, s_at, n = _u64(seqs)
+        r, r_at, n_rows = _u64(rows)
+        if n != n_rows:
             raise ValueError("one row count per sequence")
-        _ok(self._lib.kernrt_cuda_pages_step(self._ctx, pages, _ptr(s), _ptr(r), s.size))
+        _ok(self._lib.kernrt_cuda_pages_step(self._ctx, pages, s_at, r_at, n))
 
     def pages_write(self, pages: int, layer: int, k: int, v: int) -> None:
         _ok(self._lib.kernrt_cuda_pages_write(self._ctx, pages, layer, k, v))

@@ -2273,14 +2273,14 @@ namespace krt {
 void set_last_error(const std::string &msg) { g_last_error = msg; }
 }  // namespace krt
 
+// A call's errors as codes, for calls that reach no device.
 template <class F>
-static int guard(kernrt_cuda_ctx *ctx, F &&fn) {
+static int guard_host(kernrt_cuda_ctx *ctx, F &&fn) {
     if (!ctx || !ctx->b) {
         g_last_error = "null kernrt_cuda context";
         return KERNRT_E_INVALID;
     }
     try {
-        ctx->b->activate();
         fn(*ctx->b);
         return KERNRT_OK;
     } catch (const krt::Error &e) {
@@ -2290,6 +2290,15 @@ static int guard(kernrt_cuda_ctx *ctx, F &&fn) {
         g_last_error = e.what();
         return KERNRT_E_CUDA;
     }
+}
+
+// The same with the context's device made current.
+template <class F>
+static int guard(kernrt_cuda_ctx *ctx, F &&fn) {
+    return guard_host(ctx, [&](krt::Backend &b) {
+        b.activate();
+        fn(b);
+    });
 }
 
 extern "C" {
@@ -2645,7 +2654,7 @@ int kernrt_cuda_pages_ptr(kernrt_cuda_ctx *ctx, kernrt_pages pages, kernrt_pages
 }
 
 int kernrt_cuda_seq_open(kernrt_cuda_ctx *ctx, kernrt_pages pages, uint64_t *seq) {
-    return guard(ctx, [&](krt::Backend &b) {
+    return guard_host(ctx, [&](krt::Backend &b) {
         if (!seq) krt::fail(KERNRT_E_INVALID, "null output pointer");
         *seq = krt::Backend::paging([&] { return b.cache(pages).map->open(); });
     });
@@ -2653,7 +2662,7 @@ int kernrt_cuda_seq_open(kernrt_cuda_ctx *ctx, kernrt_pages pages, uint64_t *seq
 
 int kernrt_cuda_seq_fork(kernrt_cuda_ctx *ctx, kernrt_pages pages, uint64_t seq, size_t length, size_t n,
                          uint64_t *children) {
-    return guard(ctx, [&](krt::Backend &b) { b.seq_fork(pages, seq, length, n, children); });
+    return guard_host(ctx, [&](krt::Backend &b) { b.seq_fork(pages, seq, length, n, children); });
 }
 
 int kernrt_cuda_seq_copy(kernrt_cuda_ctx *ctx, kernrt_pages pages, uint64_t seq, size_t length, uint64_t *copy) {
@@ -2664,16 +2673,16 @@ int kernrt_cuda_seq_copy(kernrt_cuda_ctx *ctx, kernrt_pages pages, uint64_t seq,
 }
 
 int kernrt_cuda_seq_trim(kernrt_cuda_ctx *ctx, kernrt_pages pages, uint64_t seq, size_t length) {
-    return guard(ctx, [&](krt::Backend &b) { b.seq_trim(pages, seq, length); });
+    return guard_host(ctx, [&](krt::Backend &b) { b.seq_trim(pages, seq, length); });
 }
 
 int kernrt_cuda_seq_close(kernrt_cuda_ctx *ctx, kernrt_pages pages, const uint64_t *seqs, size_t n) {
-    return guard(ctx, [&](krt::Backend &b) { b.seq_close(pages, seqs, n); });
+    return guard_host(ctx, [&](krt::Backend &b) { b.seq_close(pages, seqs, n); });
 }
 
 int kernrt_cuda_seq_table(kernrt_cuda_ctx *ctx, kernrt_pages pages, uint64_t seq, size_t *length, int32_t *table,
                           size_t capacity, size_t *n_pages) {
-    return guard(ctx, [&](krt::Backend &b) {
+    return guard_host(ctx, [&](krt::Backend &b) {
         const krt::PageMap &m = *b.cache(pages).map;
         const krt::PageMap::Seq &q = m.at(krt::Backend::paging([&] { return m.slot(seq); }));
         if (length) *length = q.len;

@@ -403,8 +403,8 @@ int kernrt_cuda_attention(kernrt_cuda_ctx *ctx, kernrt_buf q, kernrt_buf out, ke
  * order, whatever kernrt_cuda_set_exact says.
  *
  * A layer call's launches belong to its step: captured into a graph, they are
- * valid for replays within that step only (and the step's first attention call,
- * which lays its plan down, is made before the capture).
+ * valid for replays within that step only, one after the other (and the step's
+ * first attention call, which lays its plan down, is made before the capture).
  *
  * Failures of the bookkeeping change nothing: KERNRT_E_STATE when the pool has
  * too few pages or sequences left, KERNRT_E_INVALID for bad arguments (a closed

@@ -7,6 +7,10 @@
 // distribution: its log probabilities and entropy are NaN.  The order of the
 // top entries is by value, NaN above +inf, ids ascending among equals (-0 and
 // +0 are equal).
+//
+// One read of the logits.  Measured: 1024 rows of 49152, 201 MB, 37.4 us without
+// top entries (5.4 TB/s), 52.1 us with 5; one row of 151936, 7.5 us and, with 20,
+// 12.7 us.
 #include "kernels.cuh"
 #include "paged.cuh"
 
@@ -71,8 +75,9 @@ __device__ __forceinline__ void take_top(const u64 *cand, int n, int top, F &&to
     }
 }
 
-// A bound that at least `top` of the block's best[] reach and not many more (0 if fewer than `top` are above 0): one warp bisects, the values first
-// and, where too many are equal, their ids.
+// A bound that at least `top` of the block's best[] reach and not many more (0 if
+// fewer than `top` are above 0): one warp bisects, the values first and, where
+// too many are equal, their ids.
 template <class T>
 __device__ __forceinline__ bool bisect(const T (&b)[kThreads / 32], T &lo, T hi, int top) {
     while (lo < hi) {  // at least `top` reach lo, fewer reach hi + 1

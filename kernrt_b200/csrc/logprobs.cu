@@ -288,6 +288,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(const float *__restric
             value = key_value((uint32_t)(bound >> 32));
             if (__syncthreads_count(odd || !(own < value)) > top + top / 4 + 4) raise(best_of(at, v, own, odd));
             const int n = n_cand;
+            __syncthreads();  // all have read it before any thread appends
             if (n + kNew > kRoom) {
                 take_top(cand, n, top, [&](int i, u64 k) { kept[i] = k; });
                 __syncthreads();
@@ -370,6 +371,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(const float *__restric
                 __syncthreads();
                 narrow();
                 const int n = n_cand;
+                __syncthreads();  // all have read it before the next batch comes
                 if (n > top && at + batch < total) {
                     take_top(cand, n, top, [&](int i, u64 k) { kept[i] = k; });
                     __syncthreads();

@@ -110,6 +110,25 @@ def test_large_entries_spread_evenly_over_a_row(gpu):
         check(gpu, x, [5], 64)
 
 
+@pytest.mark.parametrize("vocab", [49152, 600000, 2000001])
+def test_many_candidates_every_time_alike(gpu, vocab):
+    """Ascending rows (more entries reach the first bound than there is room for)
+    and lists of many stretches (more than one batch of them in the join), over and
+    over: threads that disagree about how many entries there are would show."""
+    rng = np.random.default_rng(vocab)
+    x = np.stack([np.arange(vocab) / 1024, rng.permutation(vocab) / 1024]).astype(np.float32)
+    want = plain(x, [0, vocab - 1], 64)
+    first = None
+    for _ in range(20):
+        got = call(gpu, x, [0, vocab - 1], 64)
+        assert np.array_equal(got[2], want[2])
+        first = first or got
+        assert all(np.array_equal(a, b) for a, b in zip(got, first))
+    near(first[0], want[0], "logprob")
+    near(first[1], want[1], "entropy")
+    near(first[3], want[3], "top log probabilities")
+
+
 def test_masked_rows_and_rows_without_a_distribution(gpu):
     rng = np.random.default_rng(3)
     x = (3 * rng.standard_normal((9, 3001))).astype(np.float32)

@@ -405,6 +405,9 @@ int kernrt_cuda_attention(kernrt_cuda_ctx *ctx, kernrt_buf q, kernrt_buf out, ke
  * A layer call's launches belong to its step: captured into a graph, they are
  * valid for replays within that step only, one after the other (and the step's
  * first attention call, which lays its plan down, is made before the capture).
+ * Calls that cannot be replayed (pages_create, _destroy, _step, _compact, seq_copy,
+ * a step's first attention, kernrt_cuda_free) fail with KERNRT_E_STATE inside a
+ * capture of the context's stream and change nothing.
  *
  * Failures of the bookkeeping change nothing: KERNRT_E_STATE when the pool has
  * too few pages or sequences left, KERNRT_E_INVALID for bad arguments (a closed
@@ -479,7 +482,9 @@ int kernrt_cuda_pages_attention(kernrt_cuda_ctx *ctx, kernrt_pages pages, size_t
  * Logits of -inf have probability 0.  A row holding NaN or +inf, or only -inf,
  * has no distribution: its outputs are NaN (its top ids still ordered by value,
  * NaN first).  A target outside the vocabulary gives NaN and KERNRT_E_DEVICE at
- * the next barrier. */
+ * the next barrier.  Captured into graphs, which replay one after the other and not
+ * beside other calls of the context, it needs scratch that an earlier call of at
+ * least its size has made: otherwise KERNRT_E_STATE. */
 #define KERNRT_TOP_MAX 64
 int kernrt_cuda_logprobs(kernrt_cuda_ctx *ctx, kernrt_buf logits, size_t rows, size_t vocab, kernrt_buf targets,
                          kernrt_buf logprob, kernrt_buf entropy, size_t top, kernrt_buf top_ids,

@@ -95,6 +95,7 @@ public:
         cudaFree(att_scratch_);
         for (auto &c : caches_) free_cache(c);
         for (Grown *g : {&lp_parts_, &lp_lists_, &lp_count_}) cudaFree(g->ptr);
+        for (void *p : kept_) cudaFree(p);
         drop_spare(0);
         cudaFree(d_err_);
         cudaFree(d_ticket_);
@@ -407,9 +408,21 @@ public:
     // Gives a buffer's memory back; its handle is not used again.
     void free_buf(kernrt_buf h) {
         Buffer &b = buf(h);
+        not_captured("free");
         flush();
         give_block(b.ptr, b.bytes);
         b = Buffer{};
+    }
+
+    bool capturing() {
+        cudaStreamCaptureStatus now = cudaStreamCaptureStatusNone;
+        check(cudaStreamIsCapturing(stream_, &now), "cudaStreamIsCapturing");
+        return now != cudaStreamCaptureStatusNone;
+    }
+    // For calls whose work cannot be replayed: they upload host memory that is
+    // used again, or make or give back memory.
+    void not_captured(const char *what) {
+        if (capturing()) fail(KERNRT_E_STATE, std::string(what) + " inside a stream capture");
     }
 
     // Device memory by size, for buffers and caches that come and go: a freed
@@ -1430,6 +1443,18 @@ public:
         return true;
     }
 
+    // The same for scratch that captured calls may hold: what it outgrows stays
+    // until the backend goes (doubling bounds that by what is in use).
+    bool grow_kept(Grown &g, size_t bytes) {
+        if (bytes <= g.bytes) return false;
+        not_captured("scratch that grows (make a call of this size before)");
+        const size_t size = std::max(bytes, 2 * g.bytes);
+        void *p = take_block(size, "cudaMalloc(scratch)");
+        if (g.ptr) kept_.push_back(g.ptr);
+        g = Grown{p, size};
+        return true;
+    }
+
     uint64_t pages_create(int kind, size_t n_layers, size_t n_heads, size_t n_kv_heads, size_t head_size,
                           size_t page_size, size_t n_pages, size_t max_seqs, size_t max_len) {
         if (kind != KERNRT_F32 && kind != KERNRT_BF16) fail(KERNRT_E_INVALID, "pages are f32 or bf16");
@@ -1447,6 +1472,7 @@ public:
         if (n_layers * 2 * n_kv_heads * page_size > big / n_pages) fail(KERNRT_E_INVALID, "page cache too large");
         const size_t max_pages = (max_len + page_size - 1) / page_size;
         if (max_pages > big / max_seqs) fail(KERNRT_E_INVALID, "page tables too large");
+        not_captured("pages_create");
         flush();
         PagedCache c;
         c.map = std::make_unique<PageMap>(n_pages, page_size, max_seqs, max_len);
@@ -1486,6 +1512,7 @@ public:
 
     void pages_destroy(uint64_t h) {
         PagedCache &c = cache(h);
+        not_captured("pages_destroy");
         flush();
         free_cache(c);
     }
@@ -1517,6 +1544,7 @@ public:
 
     uint64_t seq_copy(uint64_t h, uint64_t seq, size_t length) {
         PagedCache &c = cache(h);
+        not_captured("seq_copy");
         flush();
         std::vector<PageCopy> copies;
         const uint64_t got = paging([&] { return c.map->copy(seq, length, &copies); });
@@ -1540,6 +1568,7 @@ public:
 
     size_t pages_compact(uint64_t h) {
         PagedCache &c = cache(h);
+        not_captured("pages_compact");
         flush();
         const std::vector<PageCopy> moves = c.map->compact();
         if (!moves.empty()) c.stepped = false;
@@ -1671,6 +1700,7 @@ public:
     // Plans the step's attention and lays the pieces down for its layers
     // (counters start, and stay between launches, at 0).
     void plan_step(PagedCache &c) {
+        not_captured("the step's first pages_attention");
         const AttnPlan a = plan_attention(c.view, c.step);
         const size_t hk = (size_t)c.view.kv_heads, row = (size_t)c.view.head * sizeof(float);
         std::vector<AttnItem> items = a.decode;
@@ -1702,6 +1732,7 @@ public:
             total += (size_t)rows[i];
         }
         fits_int(total * (size_t)std::max(2, c.view.group), "pages_step");
+        not_captured("pages_step");
         flush();
         std::vector<PageCopy> copies;
         paging([&] { c.map->extend(seqs, rows, n, &copies); });
@@ -1814,9 +1845,9 @@ public:
         const size_t chunks = rows ? (size_t)logprobs_chunks((int)rows, (int)vocab) : 0;
         fits_int(rows * chunks, "logprobs");
         if (chunks > 1) {
-            grow(lp_parts_, rows * chunks * 16);
-            grow(lp_lists_, rows * chunks * top * 8);
-            if (grow(lp_count_, rows * sizeof(unsigned)))
+            grow_kept(lp_parts_, rows * chunks * 16);
+            grow_kept(lp_lists_, rows * chunks * top * 8);
+            if (grow_kept(lp_count_, rows * sizeof(unsigned)))
                 check(cudaMemsetAsync(lp_count_.ptr, 0, lp_count_.bytes, stream_), "cudaMemset");
         }
         launch_or_fail(launch_logprobs(f(xb), (int)rows, (int)vocab, ints(targets), floats(logprob), floats(entropy),
@@ -2224,6 +2255,7 @@ private:
     std::vector<DevMatrix> mats_;
     std::vector<PagedCache> caches_;
     Grown lp_parts_, lp_lists_, lp_count_;  // logprobs' scratch
+    std::vector<void *> kept_;              // what it outgrew
     std::vector<Buffer> spare_;  // freed blocks, oldest first
     size_t spare_bytes_ = 0;
     float *kc_ = nullptr, *vc_ = nullptr;

@@ -204,3 +204,65 @@ def test_refusals(gpu):
         assert e.value.code == kernrt_b200.E_INVALID, args
     gpu.logprobs(x, 0, 100, t, o[0], o[1], 3, o[2], o[3])  # no rows: nothing
     gpu.logprobs(x, 10, 100)                               # no outputs: nothing
+
+
+def test_graphs_keep_their_scratch(gpu):
+    """Captured calls of several sizes replay after larger calls have made larger
+    scratch; a capture that would have to make some is refused."""
+    import torch
+
+    from kernrt_b200.interop import as_torch
+
+    rng = np.random.default_rng(17)
+    with kernrt_b200.CudaBackend(0) as b:
+        stream = torch.cuda.ExternalStream(b.stream())
+
+        def case(rows, vocab, top):
+            x = (3 * rng.standard_normal((rows, vocab))).astype(np.float32)
+            t = rng.integers(0, vocab, rows)
+            hs = [b.upload(x), b.upload_bytes(t.astype(np.int32)), b.alloc(rows), b.alloc(rows), b.alloc(rows * top),
+                  b.alloc(rows * top)]
+            return hs, (rows, vocab, top), plain(x, t, top)
+
+        def go(hs, size):
+            b.logprobs(hs[0], size[0], size[1], hs[1], hs[2], hs[3], size[2], hs[4], hs[5])
+
+        def held(hs, size, want):
+            rows, _, top = size
+            near(b.read(hs[2], rows), want[0], "logprob")
+            near(b.read(hs[3], rows), want[1], "entropy")
+            assert np.array_equal(b.read_bytes(hs[4], 4 * rows * top, np.int32).reshape(rows, top), want[2])
+
+        cases = [case(1, 20000, 3), case(3, 49152, 20), case(5, 300001, 64)]
+        graphs = []
+        for hs, size, want in cases:
+            go(hs, size)
+            held(hs, size, want)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                go(hs, size)
+            graphs.append(g)
+        big = case(40, 151936, 64)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            go(*cases[2][:2])
+            with pytest.raises(KernrtCudaError) as e:
+                go(*big[:2])
+        assert e.value.code == kernrt_b200.E_STATE
+        for _ in range(3):
+            go(*big[:2])
+            held(*big)
+            spare = [b.alloc(n) for n in (4, 64, 1024, 16384)]  # where given-back scratch would go
+            for hs, size, _ in cases:
+                for h, n in zip(hs[2:], (size[0], size[0], size[0] * size[2], size[0] * size[2])):
+                    as_torch(b, h, (n,)).zero_()
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                for g in graphs:
+                    g.replay()
+            torch.cuda.synchronize()
+            for c in cases:
+                held(*c)
+            for h, n in zip(spare, (4, 64, 1024, 16384)):
+                assert not b.read(h, n).any()
+                b.free(h)

@@ -373,6 +373,46 @@ def test_layer_calls_replay_in_a_graph(gpu, kind):
                 assert np.array_equal(gpu.read(hs[3], rows * 2048), w)
 
 
+def test_calls_that_cannot_be_replayed_are_refused_in_a_capture(gpu):
+    """They change nothing, and the capture goes on."""
+    import torch
+
+    from kernrt_b200.interop import as_torch
+
+    rng = np.random.default_rng(83)
+    with Pair(gpu, kernrt_b200.BF16, 4, 2, 64, 16, 60, 6, 300) as c:
+        a, b = c.open(), c.open()
+        c.step([a, b], [40, 20], [c.rows(rng, 60)])
+        gpu.pages_step(c.p, [a, b], [1, 30])
+        q, k, v = [c.up(x) for x in c.rows(rng, 31)]
+        out, spare = c.up(np.zeros((31, 256), np.float32)), gpu.alloc(5)
+        gpu.pages_write(c.p, 0, k, v)
+        gpu.synchronize()
+        free, stream = gpu.pages_ptr(c.p).available, torch.cuda.ExternalStream(gpu.stream())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            gpu.pages_write(c.p, 0, k, v)
+            for call in (lambda: gpu.pages_attention(c.p, 0, q, out), lambda: gpu.pages_step(c.p, [a], [1]),
+                         lambda: gpu.seq_copy(c.p, a, 10), lambda: gpu.pages_compact(c.p),
+                         lambda: gpu.pages_destroy(c.p), lambda: gpu.free(spare),
+                         lambda: gpu.pages_create(kernrt_b200.F32, 1, 1, 1, 8, 16, 2, 1, 16)):
+                with pytest.raises(KernrtCudaError) as e:
+                    call()
+                assert e.value.code == kernrt_b200.E_STATE and "capture" in str(e.value)
+        assert gpu.pages_ptr(c.p).available == free
+        assert len(gpu.seq_table(c.p, a)) == 3 and len(gpu.seq_table(c.p, b)) == 4
+        gpu.pages_attention(c.p, 0, q, out)  # the step stands
+        want = gpu.read(out, 31 * 256)
+        as_torch(gpu, out, (31 * 256,)).zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            g.replay()
+        torch.cuda.synchronize()
+        gpu.pages_attention(c.p, 0, q, out)
+        assert np.array_equal(gpu.read(out, 31 * 256), want)
+        gpu.free(spare)
+
+
 def test_freed_memory_comes_back_zeroed(gpu):
     """A freed block serves the next allocation of its size, behind the work that
     still uses it."""

@@ -22,12 +22,13 @@
 // for more, because the tile's largest may stand in a row that is masked or has
 // no weight: where some group of neighbouring values (four of bf16, eight of
 // f32) lies 2^28 (f32: 2^20) below the tile's largest, and above 2^-60 all the
-// same, the CTA's rows are attended again by attend_row in f32, each over the
-// keys it sees alone.  So they are where a tile or a query holds an infinity, and
-// so are rows whose result is not finite, unless their sum of weights is NaN: that
-// takes a NaN score the row does see, and the row is NaN.  What stands in masked
-// places (later positions of the same prompt included) therefore never reaches a
-// row.  (NaN stays out of the tiles' largest.)
+// same, the rows that see some of the tile are attended again by attend_row in
+// f32, each over the keys it sees alone.  So they are where the tile or their query
+// holds an infinity, and so are rows whose result is not finite, unless their sum
+// of weights is NaN: that takes a NaN score the row does see, and the row is NaN.
+// The marks travel with the tiles' scales (a negative scale of V, an infinite one
+// of K), so that they reach the same rows every time, however far ahead the loader
+// is.  (NaN stays out of the tiles' largest.)
 // The tensor cores add into an f32 accumulator with truncation: measured
 // relative error 1.1e-9 per K (9e-6 at K = 8192, always toward zero), so
 // a tile's sum of V is taken out of TMEM after every 64 or 128 keys and added in
@@ -328,7 +329,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     __shared__ uint64_t slot_full[S::Slots], slot_empty[S::Slots], s_full[3], p_full[2], o_full[2], o_free, q_full, done;
     __shared__ uint32_t s_tmem, s_red[2][4][2];
     __shared__ float s_kscale[kScaleRing], s_vscale[kScaleRing];
-    __shared__ int s_abort, s_wild;
+    __shared__ int s_abort;
     const uint32_t base = (smem_addr(raw_smem) + 1023u) & ~1023u;
     const uint32_t slots = base + 2 * S::QTile;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -348,7 +349,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         mbar_init(&q_full, 8);
         mbar_init(&done, 1);
         s_abort = 0;
-        s_wild = 0;
         mbar_fence_init();
     }
     if (warp == 12) {
@@ -411,9 +411,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             uint32_t most = 0;
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) most = max(most, most_of(x[2 * c], x[2 * c + 1]));
-            if (most == 0x7f800000u) s_wild = 1;
             const float up = up_scale(most);
-            sc = kLog2e * rsqrtf((float)p.head) * down_scale(up);
+            sc = most == 0x7f800000u ? INFINITY : kLog2e * rsqrtf((float)p.head) * down_scale(up);
             const uint32_t tile = base + (uint32_t)t * S::QTile;
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) {
@@ -432,13 +431,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
         for (int d = 0; d < D / 2; ++d) acc[d] = both(0.0f);
         float m = -INFINITY, l = 0.0f;
+        bool again = false;  // the row is attended again in f32
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t o_at = tmem + lanes + (uint32_t)(S::SumAt + (S::Sums == 2 ? t * D : 0));
         // the sum of V over a key tile, once it is there, into the registers
         const auto flush = [&](int tile) {
             if (!__all_sync(0xffffffffu, wait(&o_full[t], (uint32_t)tile & 1u))) return false;
             tc_fence_after();
-            const float vs = s_vscale[tile & (kScaleRing - 1)];
+            const float mark = s_vscale[tile & (kScaleRing - 1)], vs = fabsf(mark);
+            again = again || (mark < 0.0f && limit > it.lo + tile * Keys);
             tmem_each<D, W>(o_at, [&](int c, uint32_t(&v)[W]) {
 #pragma unroll
                 for (int i = 0; i < W / 2; ++i)
@@ -465,6 +466,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             const int rem = limit - (it.lo + tile * Keys);  // the tile's keys this row sees
             const bool masked = __any_sync(0xffffffffu, rem < Keys);
             const float ks = sc * s_kscale[tile & (kScaleRing - 1)];
+            again = again || (rem > 0 && ks == INFINITY);
             float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             // (rolled loops: the roles' code competes for the instruction caches)
 #pragma unroll 1
@@ -529,7 +531,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
             for (int d = 0; d < D / 2; ++d) fine = fine && isfinite(acc[d].x) && isfinite(acc[d].y);
             fine = fine || l != l;  // (a NaN score among the row's own: dividing by l says so)
-            fine = fine && !*(volatile int *)&s_wild;
+            fine = fine && !again;
             const size_t part = ((size_t)item * p.kv_heads + j) * kRows + r;
             if (live && fine) {
                 const float f = it.n_parts == 1 ? 1.0f / l : 0x1p-14f;
@@ -540,10 +542,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                         dst[d / 2] = make_float4(acc[d].x * f, acc[d].y * f, acc[d + 1].x * f, acc[d + 1].y * f);
                 if (it.n_parts > 1) scratch.ml[part] = make_float2(m, l * 0x1p-14f);
             }
-            unsigned again = __ballot_sync(0xffffffffu, live && !fine);
-            while (again) {
-                const int w = __ffs((int)again) - 1;
-                again &= again - 1;
+            unsigned rest = __ballot_sync(0xffffffffu, live && !fine);
+            while (rest) {
+                const int w = __ffs((int)rest) - 1;
+                rest &= rest - 1;
                 const size_t at_w = __shfl_sync(0xffffffffu, at, w), part_w = __shfl_sync(0xffffffffu, part, w);
                 const RowAcc a = attend_row(p, layer, j, table, q + at_w, it.lo, __shfl_sync(0xffffffffu, limit, w));
 #pragma unroll
@@ -641,8 +643,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
             const float up = up_scale(most);
             if (tid == 0) {
-                if (most == 0x7f800000u || (is_v(i) && too_wide(most, least, F32 ? 20 : 28))) s_wild = 1;
-                (is_v(i) ? s_vscale : s_kscale)[tile_of(i) & (kScaleRing - 1)] = down_scale(up);
+                const bool inf = most == 0x7f800000u, mark = inf || too_wide(most, least, F32 ? 20 : 28);
+                const float down = down_scale(up);
+                if (is_v(i)) s_vscale[tile_of(i) & (kScaleRing - 1)] = mark ? -down : down;
+                else s_kscale[tile_of(i) & (kScaleRing - 1)] = inf ? INFINITY : down;
             }
             const uint32_t dst =
                 slots + (uint32_t)slot * S::Slot + (uint32_t)(chunk >> 3) * S::Sub + swizzled(row, chunk & 7);

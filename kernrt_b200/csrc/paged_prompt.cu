@@ -17,14 +17,15 @@
 // tile's largest, and f32 values (as two halves, three products) to 2^-22 of
 // their own or 2^-39 of the tile's largest, whichever is more; query rows
 // likewise, row by row.  The scales return as one factor of the scores and one of
-// the tile's sum.  A score only needs its absolute error small, and 2^-39 of the
-// largest query and key is far below the rounding of f32 sums.  Values are asked
-// for more, because the tile's largest may stand in a row that is masked or has
-// no weight: where some group of neighbouring values (four of bf16, eight of
+// the tile's sum.  A score only needs its absolute error small, and the row's and
+// the tile's largest bound it, whether or not they meet in a score that counts: it
+// is below 2^-18 while their product stays below 2^14 (heads of 128; 2^15 for 64).
+// Beyond, the row is attended again by attend_row in f32, over the keys it sees
+// alone.  Values are asked for more, because the tile's largest may stand in a
+// row that is masked or has no weight: where some group of neighbouring values (four of bf16, eight of
 // f32) lies 2^28 (f32: 2^20) below the tile's largest, and above 2^-60 all the
-// same, the rows that see some of the tile are attended again by attend_row in
-// f32, each over the keys it sees alone.  So they are where the tile or their query
-// holds an infinity, and so are rows whose result is not finite, unless their sum
+// same, the rows that see some of the tile are attended again, too.  So they are
+// where the tile or their query holds an infinity, and so are rows whose result is not finite, unless their sum
 // of weights is NaN: that takes a NaN score the row does see, and the row is NaN.
 // The marks travel with the tiles' scales (a negative scale of V, an infinite one
 // of K), so that they reach the same rows every time, however far ahead the loader
@@ -61,6 +62,11 @@ namespace {
 
 constexpr int kRows = kPromptRows;  // query rows of a CTA
 constexpr int kPromptThreads = 512;
+// Largest factor of the scores, times the head size, that the halves carry: an
+// element far below its row's (its tile's) largest is off by up to 2^-25, times
+// 2^14 at most and twice for q and K makes 2^-10 an element of the head before the
+// factor, and 2^-18 (in powers of two) of the score with this one.
+constexpr float kScoreTop = 0x1p-8f;
 constexpr int kScaleRing = 16;  // tiles' scales; the loader is at most 4 tiles ahead
 
 template <int D, bool F32>
@@ -400,7 +406,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const size_t at =
             ((size_t)(sq.row0 + token) * p.heads + (size_t)j * p.group + (m_row - token * p.group)) * p.head;
         const int limit = live ? min(it.hi, sq.ctx + token + 1) : it.lo;
-        float sc;
+        float down;  // the scale of the row's halves, taken back
         {  // the row's halves, scaled to its largest element
             const int chunks = p.head >> 3;
             const float4 *src = reinterpret_cast<const float4 *>(q + at);
@@ -412,7 +418,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) most = max(most, most_of(x[2 * c], x[2 * c + 1]));
             const float up = up_scale(most);
-            sc = most == 0x7f800000u ? INFINITY : kLog2e * rsqrtf((float)p.head) * down_scale(up);
+            down = most == 0x7f800000u ? INFINITY : down_scale(up);
             const uint32_t tile = base + (uint32_t)t * S::QTile;
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) {
@@ -465,8 +471,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             if (buf >= 3) buf -= 3, round ^= 1;
             const int rem = limit - (it.lo + tile * Keys);  // the tile's keys this row sees
             const bool masked = __any_sync(0xffffffffu, rem < Keys);
-            const float ks = sc * s_kscale[tile & (kScaleRing - 1)];
-            again = again || (rem > 0 && ks == INFINITY);
+            // (the powers of two first: their product is exact, or far out of use)
+            const float ks = kLog2e * rsqrtf((float)p.head) * (down * s_kscale[tile & (kScaleRing - 1)]);
+            again = again || (rem > 0 && !(ks * (float)p.head <= kScoreTop));
             float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             // (rolled loops: the roles' code competes for the instruction caches)
 #pragma unroll 1

@@ -1,17 +1,50 @@
 """Attention of many query rows over keys, queries and values of very different
 size: what is large, masked or infinite in one place leaves the rest of its tile
 as it is by the definition.
+
+The bound, per output element, with p_t the weights, v_t the values and o the
+output in 64 bits.  A score of key t is off by at most dx_t = (3 * 2^-22 + D 2^-23)
+sum |q k_t| / sqrt(D), as in tests/_paged.py but of its own key, and 2^-18 for what
+16-bit halves lose far below a tile's or a row's largest element; that moves o by
+at most sum p_t e_t |v_t - o| with e_t = exp(dx_t) - 1, doubled for the terms of
+second order.  Everything else acts on sum p |v|: 2^-18 as there, once more for
+values far below a tile's largest, 3 * 2^-22 and 32 * 2^-23 as there, and the
+additions: n / 64 + 16 of tiles and pieces where the tensor cores take the tiles,
+n one by one where the rows are attended in f32, 2^-24 each.
 """
+import math
+
 import numpy as np
 import pytest
 
 from kernrt_b200 import BF16, F32
-from tests._paged import Pair
+from tests._paged import Pair, rounded, same
 
 pytestmark = pytest.mark.gpu
 
 KINDS = pytest.mark.parametrize("kind", [BF16, F32], ids=["bf16", "f32"])
 D = 128
+
+
+def check(c, data, out, rows, heads, by_one=True):
+    """Some rows of a first step of one sequence."""
+    q, k, v = data
+    n = len(q)
+    q = q.astype(np.float64).reshape(n, c.heads, D)
+    k, v = (rounded(x, c.kind).reshape(n, c.kv_heads, D) for x in (k, v))
+    for r in rows:
+        m = r + 1
+        adds = (m if by_one else m / 64) + 16
+        rest = 2 * 2.0 ** -18 + 3 * 2.0 ** -22 + 32 * 2.0 ** -23 + adds * 2.0 ** -24
+        for h in heads:
+            kj, vj = k[:m, h * c.kv_heads // c.heads], v[:m, h * c.kv_heads // c.heads]
+            x = kj @ q[r, h] / math.sqrt(D)
+            dx = np.abs(kj) @ np.abs(q[r, h]) / math.sqrt(D) * (3 * 2.0 ** -22 + D * 2.0 ** -23) + 2.0 ** -18
+            p = np.exp(x - x.max())
+            p /= p.sum()
+            o = p @ vj
+            bound = 2 * (p * np.expm1(np.minimum(dx, 50))) @ np.abs(vj - o) + rest * (p @ np.abs(vj))
+            same(out[r, h], o, bound, f"row {r} head {h}")
 
 
 def attend(gpu, kind, data, heads=16, kv_heads=8):
@@ -39,3 +72,51 @@ def test_an_infinity_leaves_the_query_tiles_before_it_bit_for_bit(gpu, kind):
                 c, got = attend(gpu, kind, data, 16, 16)
                 first = at // 128 * 128
                 assert np.array_equal(got[:first], want[:first]), (at, put, which)
+
+
+@KINDS
+@pytest.mark.parametrize("scale", [1e6, 1e8, 1e12, 1e30], ids=str)
+def test_a_large_key_leaves_the_rows_before_it(gpu, kind, scale):
+    data = normal(2)
+    data[1][400] *= scale
+    c, out = attend(gpu, kind, data)
+    check(c, data, out, [272, 300, 383, 384, 390, 399, 400, 401, 511, 900], [0, 3, 15])
+
+
+@KINDS
+@pytest.mark.parametrize("scale", [1e6, 1e12, 1e30], ids=str)
+def test_a_large_key_across_the_query(gpu, kind, scale):
+    """Large where every query is 0."""
+    data = normal(3)
+    data[0][:, 17::D] = 0
+    data[1][400, 17::D] = scale
+    data[1][700:, 17::D] = -scale
+    c, out = attend(gpu, kind, data)
+    check(c, data, out, [390, 399, 400, 401, 511, 699, 700, 1099], [0, 3, 15])
+
+
+@KINDS
+@pytest.mark.parametrize("scale", [1e6, 1e12, 1e30], ids=str)
+def test_a_large_query_element_across_the_keys(gpu, kind, scale):
+    """Large where every key is 0, in some rows."""
+    data = normal(4)
+    data[1][:, 17::D] = 0
+    data[0][::3, 17::D] = scale
+    c, out = attend(gpu, kind, data)
+    check(c, data, out, [0, 1, 300, 301, 900, 901], [0, 3, 15])
+
+
+@KINDS
+def test_scales_whose_product_leaves_f32(gpu, kind):
+    """Queries of 1e30 where keys are 0 and keys of 1e20 where queries are 0: the
+    scores are ordinary.  And queries of 1e-36 before keys of 1e36."""
+    data = normal(5)
+    data[0][:, 0::D], data[1][:, 0::D] = 1e30, 0
+    data[0][:, 1::D], data[1][:, 1::D] = 0, 1e20
+    c, out = attend(gpu, kind, data)
+    check(c, data, out, [0, 255, 256, 777, 1099], [0, 9, 15])
+    data = normal(6)
+    data[0] *= np.float32(1e-36)
+    data[1] *= np.float32(1e36)
+    c, out = attend(gpu, kind, data)
+    check(c, data, out, [0, 255, 256, 777, 1099], [0, 9, 15], by_one=False)

@@ -22,11 +22,12 @@
 // is below 2^-18 while their product stays below 2^14 (heads of 128; 2^15 for 64).
 // Beyond, the row is attended again by attend_row in f32, over the keys it sees
 // alone.  Values are asked for more, because the tile's largest may stand in a
-// row that is masked or has no weight: where some group of neighbouring values (four of bf16, eight of
-// f32) lies 2^28 (f32: 2^20) below the tile's largest, and above 2^-60 all the
-// same, the rows that see some of the tile are attended again, too.  So they are
-// where the tile or their query holds an infinity, and so are rows whose result is not finite, unless their sum
-// of weights is NaN: that takes a NaN score the row does see, and the row is NaN.
+// row that is masked or has no weight: where some group of neighbouring values
+// (four of bf16, eight of f32) lies 2^28 (f32: 2^20) below the tile's largest and
+// is not zero, the rows that see some of the tile are attended again, too.  So they
+// are where the tile or their query holds an infinity, and so are rows whose
+// result is not finite, unless their sum of weights is NaN: that takes a NaN score
+// the row does see, and the row is NaN.
 // The marks travel with the tiles' scales (a negative scale of V, an infinite one
 // of K), so that they reach the same rows every time, however far ahead the loader
 // is.  (NaN stays out of the tiles' largest.)
@@ -260,13 +261,11 @@ __device__ __forceinline__ float up_scale(uint32_t bits) {
 }
 __device__ __forceinline__ float down_scale(float up) { return __uint_as_float((254u << 23) - __float_as_uint(up)); }
 
-// Magnitudes (as f32 bits) less kTiny, unsigned: those below 2^-60, zeros among
-// them, come out above all others.
-constexpr uint32_t kTiny = 67u << 23;
 // Whether values spread too far for one scale: the largest magnitude's bits, and
-// the least of the groups' largest less kTiny.
-__device__ __forceinline__ bool too_wide(uint32_t most, uint32_t least, int bits) {
-    return least < 0x80000000u && (int)(most >> 23) - (int)((least + kTiny) >> 23) > bits;
+// the least of the groups' largest, less one (so that zeros come out above all
+// others; of bf16 one is the upper half's).
+__device__ __forceinline__ bool too_wide(uint32_t most, uint32_t least, uint32_t one, int bits) {
+    return least < 0x80000000u && (int)(most >> 23) - (int)((least + one) >> 23) > bits;
 }
 
 // The bits of the largest magnitude of eight f32 (NaN left out).
@@ -620,7 +619,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     const uint32_t m = most_of(*reinterpret_cast<const float4 *>(&v[2 * k]),
                                                *reinterpret_cast<const float4 *>(&v[2 * k + 1]));
                     most = max(most, m);
-                    least = min(least, m - kTiny);
+                    least = min(least, m - 1);
                 }
             } else {  // two bf16 a register; the chunks are the four even and the four odd elements
                 uint32_t hi = 0, lo = 0xffffffffu;
@@ -629,7 +628,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     const uint32_t m = max_bf16x2(max_bf16x2(v[k].x & 0x7fff7fffu, v[k].y & 0x7fff7fffu),
                                                   max_bf16x2(v[k].z & 0x7fff7fffu, v[k].w & 0x7fff7fffu));
                     hi = max_bf16x2(hi, m);
-                    lo = min_u16x2(lo, __vsub2(m, kTiny | kTiny >> 16));
+                    lo = min_u16x2(lo, __vsub2(m, 0x00010001u));
                 }
                 most = max(hi << 16, hi & 0xffff0000u);
                 least = min(lo << 16, lo & 0xffff0000u);
@@ -650,7 +649,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
             const float up = up_scale(most);
             if (tid == 0) {
-                const bool inf = most == 0x7f800000u, mark = inf || too_wide(most, least, F32 ? 20 : 28);
+                const bool inf = most == 0x7f800000u;
+                const bool mark = inf || too_wide(most, least, F32 ? 1 : 0x10000, F32 ? 20 : 28);
                 const float down = down_scale(up);
                 if (is_v(i)) s_vscale[tile_of(i) & (kScaleRing - 1)] = mark ? -down : down;
                 else s_kscale[tile_of(i) & (kScaleRing - 1)] = inf ? INFINITY : down;

@@ -120,3 +120,12 @@ def test_scales_whose_product_leaves_f32(gpu, kind):
     data[1] *= np.float32(1e36)
     c, out = attend(gpu, kind, data)
     check(c, data, out, [0, 255, 256, 777, 1099], [0, 9, 15], by_one=False)
+
+
+@KINDS
+@pytest.mark.parametrize("small", [1e-7, 1e-12, 1e-19, 1e-30], ids=str)
+def test_small_values_beside_masked_ones(gpu, kind, small):
+    data = normal(7)
+    data[2][:700] *= np.float32(small)
+    c, out = attend(gpu, kind, data)
+    check(c, data, out, [0, 639, 640, 650, 699, 700, 1000], [0, 9, 15])

@@ -22,10 +22,11 @@
 // is below 2^-18 while their product stays below 2^14 (heads of 128; 2^15 for 64).
 // Beyond, the row is attended again by attend_row in f32, over the keys it sees
 // alone.  Values are asked for more, because the tile's largest may stand in a
-// row that is masked or has no weight: where some group of neighbouring values
-// (four of bf16, eight of f32) lies 2^28 (f32: 2^20) below the tile's largest and
-// is not zero, the rows that see some of the tile are attended again, too.  So they
-// are where the tile or their query holds an infinity, and so are rows whose
+// row that is masked or has no weight, or in another column: where some group of
+// neighbours of a row or of a column lies more than 2^16 below the tile's largest
+// and is not zero, the rows that see some of the tile are attended again, too.  (So
+// a value is off by at most 2^-23 of the largest of its neighbours.)  So they are
+// where the tile or their query holds an infinity, and so are rows whose
 // result is not finite, unless their sum of weights is NaN: that takes a NaN score
 // the row does see, and the row is NaN.
 // The marks travel with the tiles' scales (a negative scale of V, an infinite one
@@ -261,13 +262,6 @@ __device__ __forceinline__ float up_scale(uint32_t bits) {
 }
 __device__ __forceinline__ float down_scale(float up) { return __uint_as_float((254u << 23) - __float_as_uint(up)); }
 
-// Whether values spread too far for one scale: the largest magnitude's bits, and
-// the least of the groups' largest, less one (so that zeros come out above all
-// others; of bf16 one is the upper half's).
-__device__ __forceinline__ bool too_wide(uint32_t most, uint32_t least, uint32_t one, int bits) {
-    return least < 0x80000000u && (int)(most >> 23) - (int)((least + one) >> 23) > bits;
-}
-
 // The bits of the largest magnitude of eight f32 (NaN left out).
 __device__ __forceinline__ uint32_t most_of(const float4 &a, const float4 &b) {
     const float x = fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w)));
@@ -296,16 +290,78 @@ __device__ __forceinline__ uint32_t to_half(uint32_t u, __nv_bfloat162 s) {
     u = *reinterpret_cast<const uint32_t *>(&v);
     return pack_half(pair(u << 16, u & 0xffff0000u));
 }
-// (max.bf16x2 leaves NaN out: the larger of the others)
-__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+// The larger magnitudes of two pairs, with signs of no meaning (NaN is left out).
+__device__ __forceinline__ uint32_t max_abs_bf16x2(uint32_t a, uint32_t b) {
     uint32_t d;
-    asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
 __device__ __forceinline__ uint32_t min_u16x2(uint32_t a, uint32_t b) {
     uint32_t d;
     asm("min.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
+}
+
+// How far values may spread, in powers of two: the largest of a few neighbours
+// below their tile's largest.  The neighbours are eight elements of a row (of bf16
+// the four even or the four odd ones), and a thread's N rows of a column.  (Of a
+// single row an element is no group: an ordinary one is small now and then.)
+constexpr int kSpread = 16;
+// The largest magnitude (as f32 bits) of a thread's share of a tile, eight elements
+// of each of N rows, and the least of its rows' largest, less one step of their
+// bits, so that zeros come out above all others.
+template <bool F32, int N>
+__device__ __forceinline__ void rows_spread(const uint4 (&v)[N * (F32 ? 2 : 1)], uint32_t &most, uint32_t &least) {
+    if constexpr (F32) {
+        most = 0, least = 0xffffffffu;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const uint32_t m = most_of(*reinterpret_cast<const float4 *>(&v[2 * k]),
+                                       *reinterpret_cast<const float4 *>(&v[2 * k + 1]));
+            most = max(most, m);
+            least = min(least, m - 1);
+        }
+    } else {  // two bf16 a register
+        uint32_t hi = 0, lo = 0xffffffffu;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const uint32_t m = max_abs_bf16x2(max_abs_bf16x2(v[k].x, v[k].y), max_abs_bf16x2(v[k].z, v[k].w)) & 0x7fff7fffu;
+            hi = max_abs_bf16x2(hi, m);
+            lo = min_u16x2(lo, __vsub2(m, 0x00010001u));
+        }
+        most = max(hi << 16, hi & 0xffff0000u);
+        least = min(lo << 16, lo & 0xffff0000u);
+    }
+}
+// The same least of its columns.
+template <bool F32, int N>
+__device__ __forceinline__ uint32_t columns_spread(const uint4 (&v)[N * (F32 ? 2 : 1)]) {
+    if constexpr (F32) {
+        uint32_t least = 0xffffffffu;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            float m = 0.0f;
+#pragma unroll
+            for (int k = 0; k < N; ++k) m = fmaxf(m, fabsf((&reinterpret_cast<const float4 *>(&v[2 * k + x / 4])->x)[x % 4]));
+            least = min(least, __float_as_uint(m) - 1);
+        }
+        return least;
+    } else {
+        uint32_t m[4] = {0, 0, 0, 0}, lo = 0xffffffffu;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            m[0] = max_abs_bf16x2(m[0], v[k].x), m[1] = max_abs_bf16x2(m[1], v[k].y);
+            m[2] = max_abs_bf16x2(m[2], v[k].z), m[3] = max_abs_bf16x2(m[3], v[k].w);
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) lo = min_u16x2(lo, __vsub2(m[x] & 0x7fff7fffu, 0x00010001u));
+        return min(lo << 16, lo & 0xffff0000u);
+    }
+}
+template <bool F32>
+__device__ __forceinline__ bool too_wide(uint32_t most, uint32_t least) {
+    constexpr uint32_t step = F32 ? 1 : 0x10000;
+    return least < 0x80000000u && (int)(most >> 23) - (int)((least + step) >> 23) > kSpread;
 }
 
 // Barrier of the loader's 128 threads that also says whether any of them has p.
@@ -611,30 +667,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         for (int i = 0; i < 2 * n; ++i) {
             const int next = min(i + 1, 2 * n - 1);
             const size_t place_next = places(tile_of(min(i + 2, 2 * n - 1)));
-            // the tile's largest magnitude, and the smallest of the chunks'
-            uint32_t most = 0, least = 0xffffffffu;
-            if constexpr (F32) {
-#pragma unroll
-                for (int k = 0; k < Loads; ++k) {
-                    const uint32_t m = most_of(*reinterpret_cast<const float4 *>(&v[2 * k]),
-                                               *reinterpret_cast<const float4 *>(&v[2 * k + 1]));
-                    most = max(most, m);
-                    least = min(least, m - 1);
-                }
-            } else {  // two bf16 a register; the chunks are the four even and the four odd elements
-                uint32_t hi = 0, lo = 0xffffffffu;
-#pragma unroll
-                for (int k = 0; k < Loads; ++k) {
-                    const uint32_t m = max_bf16x2(max_bf16x2(v[k].x & 0x7fff7fffu, v[k].y & 0x7fff7fffu),
-                                                  max_bf16x2(v[k].z & 0x7fff7fffu, v[k].w & 0x7fff7fffu));
-                    hi = max_bf16x2(hi, m);
-                    lo = min_u16x2(lo, __vsub2(m, 0x00010001u));
-                }
-                most = max(hi << 16, hi & 0xffff0000u);
-                least = min(lo << 16, lo & 0xffff0000u);
+            // the tile's largest magnitude and, of V, the smallest of its groups'
+            // (columns where this thread has rows, not one, or the first tile is all)
+            uint32_t most, least;
+            rows_spread<F32, Loads>(v, most, least);
+            if (is_v(i)) {
+                const int at = tile_of(i);
+                if (room_of(at) > Step || it.lo + at == 0) least = min(least, columns_spread<F32, Loads>(v));
+                least = __reduce_min_sync(0xffffffffu, least);
             }
             most = __reduce_max_sync(0xffffffffu, most);
-            least = __reduce_min_sync(0xffffffffu, least);
             uint32_t(&red)[4][2] = s_red[i & 1];
             if (lane == 0) {
                 red[warp - 8][0] = most;
@@ -650,7 +692,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             const float up = up_scale(most);
             if (tid == 0) {
                 const bool inf = most == 0x7f800000u;
-                const bool mark = inf || too_wide(most, least, F32 ? 1 : 0x10000, F32 ? 20 : 28);
+                const bool mark = inf || too_wide<F32>(most, least);
                 const float down = down_scale(up);
                 if (is_v(i)) s_vscale[tile_of(i) & (kScaleRing - 1)] = mark ? -down : down;
                 else s_kscale[tile_of(i) & (kScaleRing - 1)] = inf ? INFINITY : down;

@@ -129,3 +129,15 @@ def test_small_values_beside_masked_ones(gpu, kind, small):
     data[2][:700] *= np.float32(small)
     c, out = attend(gpu, kind, data)
     check(c, data, out, [0, 639, 640, 650, 699, 700, 1000], [0, 9, 15])
+
+
+@KINDS
+@pytest.mark.parametrize("scale", [1e5, 1e8, 1e12, 1e25], ids=str)
+@pytest.mark.parametrize("columns", [(0,), (0, 1), (6, 7)], ids=str)
+def test_large_columns_beside_ordinary_ones(gpu, kind, scale, columns):
+    """Values that are large in one or two of every eight elements, in every row."""
+    data = normal(8)
+    for x in columns:
+        data[2][:, x::8] *= np.float32(scale)
+    c, out = attend(gpu, kind, data)
+    check(c, data, out, [0, 100, 650, 1099], [0, 9, 15])

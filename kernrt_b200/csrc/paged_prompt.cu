@@ -28,7 +28,10 @@
 // a value is off by at most 2^-23 of the largest of its neighbours.)  So they are
 // where the tile or their query holds an infinity, and so are rows whose
 // result is not finite, unless their sum of weights is NaN: that takes a NaN score
-// the row does see, and the row is NaN.
+// the row does see, and the row is NaN.  Weights, carried to 2^-39 of the largest,
+// are taken relative to the largest of their row and tile, not of the row so far,
+// and the difference joins the tile's scale: large values further on may count
+// with weights far below it.
 // The marks travel with the tiles' scales (a negative scale of V, an infinite one
 // of K), so that they reach the same rows every time, however far ahead the loader
 // is.  (NaN stays out of the tiles' largest.)
@@ -492,6 +495,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
         for (int d = 0; d < D / 2; ++d) acc[d] = both(0.0f);
         float m = -INFINITY, l = 0.0f;
+        float f = 0.0f;      // the weights' own scale in the last tile, 2^(its maximum - m)
         bool again = false;  // the row is attended again in f32
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t o_at = tmem + lanes + (uint32_t)(S::SumAt + (S::Sums == 2 ? t * D : 0));
@@ -499,7 +503,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const auto flush = [&](int tile) {
             if (!__all_sync(0xffffffffu, wait(&o_full[t], (uint32_t)tile & 1u))) return false;
             tc_fence_after();
-            const float mark = s_vscale[tile & (kScaleRing - 1)], vs = fabsf(mark);
+            const float mark = s_vscale[tile & (kScaleRing - 1)], vs = f * fabsf(mark);
             again = again || (mark < 0.0f && limit > it.lo + tile * Keys);
             tmem_each<D, W>(o_at, [&](int c, uint32_t(&v)[W]) {
 #pragma unroll
@@ -546,7 +550,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
             const float mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
             if (S::Sums == 2 && tile && !(ok = flush(tile - 1))) break;
-            const float mn = fmaxf(m, mx * ks);
+            const float mt = mx * ks, mn = fmaxf(m, mt);
             if (tile && __any_sync(0xffffffffu, mn > m)) {
                 const float keep = mn == -INFINITY ? 0.0f : ex2(m - mn);
                 l *= keep;
@@ -554,8 +558,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 for (int d = 0; d < D / 2; ++d) acc[d] = mul2(acc[d], both(keep));
             }
             m = mn;
-            // weights times 2^14: the halves of small ones stay normal numbers
-            const float bias = 14.0f - (m == -INFINITY ? 0.0f : m);
+            // weights relative to the tile's own largest, times 2^14: the halves of
+            // small ones stay normal numbers (mt: -inf or NaN where the row sees no
+            // finite score)
+            const bool some = mt > -INFINITY;
+            const float bias = 14.0f - (some ? mt : 0.0f);
             F2 sum[2] = {both(0.0f), both(0.0f)};
             const auto weights = [&](auto some_masked) {
 #pragma unroll 1
@@ -580,11 +587,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             };
             if (masked) weights(Tile<1>{});
             else weights(Tile<0>{});
-            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[t]);
+            f = some ? ex2(mt - m) : 0.0f;
+            l = __fmaf_rn((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), f, l);
             if (S::Sums == 1) ok = flush(tile);
         }
         if (S::Sums == 2 && ok && mine) ok = flush(mine - 1);

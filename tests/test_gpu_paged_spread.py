@@ -141,3 +141,37 @@ def test_large_columns_beside_ordinary_ones(gpu, kind, scale, columns):
         data[2][:, x::8] *= np.float32(scale)
     c, out = attend(gpu, kind, data)
     check(c, data, out, [0, 100, 650, 1099], [0, 9, 15])
+
+
+MANY = (64, 32)  # heads and kv heads of enough pieces that none is split: a split's parts have maxima of their own
+
+
+def leveled(seed, levels, sizes):
+    """Scores next to `levels` (per key, the same for every query), values of `sizes`."""
+    q, k, v = normal(seed, len(levels), *MANY)
+    q *= np.float32(0.3)
+    k *= np.float32(0.3)
+    q[:, 0::D] = math.sqrt(D)
+    k[:, 0::D] = np.asarray(levels, np.float32)[:, None]
+    v *= np.asarray(sizes, np.float32)[:, None]
+    return [q, k, v]
+
+
+@KINDS
+@pytest.mark.parametrize("level,size", [(-14, 1e5), (-21, 1e8), (-26, 1e11), (-30, 1e12), (-60, 1e25)], ids=str)
+def test_small_weights_of_large_values(gpu, kind, level, size):
+    """One key holds nearly all the weight; a tile of others has weights of e^level
+    on values so large that they count as much."""
+    levels, sizes = np.full(1300, -80.0), np.ones(1300)
+    levels[0] = 0
+    levels[1024:1152], sizes[1024:1152] = level, size
+    data = leveled(9, levels, sizes)
+    c, out = attend(gpu, kind, data, *MANY)
+    check(c, data, out, [1023, 1100, 1151, 1152, 1290], [0, 9, 63], by_one=False)
+    # the same within a tile
+    levels, sizes = np.full(1300, -80.0), np.ones(1300)
+    levels[1030] = 0
+    levels[1031:1150], sizes[1031:1150] = level, size
+    data = leveled(10, levels, sizes)
+    c, out = attend(gpu, kind, data, *MANY)
+    check(c, data, out, [1029, 1030, 1100, 1151, 1290], [0, 9, 63])

@@ -63,9 +63,9 @@ public:
     explicit Backend(int device) : device_(device) {
         check(cudaSetDevice(device_), "cudaSetDevice");
         check(cudaStreamCreateWithFlags(&stream_, cudaStreamNonBlocking), "cudaStreamCreate");
-        check(cudaMalloc(&d_err_, sizeof(int)), "cudaMalloc(error word)");
+        device_malloc(&d_err_, sizeof(int), "cudaMalloc(error word)");
         check(cudaMemsetAsync(d_err_, 0, sizeof(int), stream_), "cudaMemset");
-        check(cudaMalloc(&d_ticket_, sizeof(unsigned)), "cudaMalloc(stream ticket)");
+        device_malloc(&d_ticket_, sizeof(unsigned), "cudaMalloc(stream ticket)");
         check(cudaMemsetAsync(d_ticket_, 0, sizeof(unsigned), stream_), "cudaMemset");
         check(cudaMallocHost(&h_err_, sizeof(int)), "cudaMallocHost");
         grow_staging(1 << 20);
@@ -152,12 +152,12 @@ public:
         const size_t n = vocab * dim;
         if (kind == KERNRT_F32 || kind == KERNRT_BF16) {
             const size_t bytes = n * (kind == KERNRT_F32 ? 4 : 2);
-            check(cudaMalloc(&emb_data_, bytes), "cudaMalloc(embedding)");
+            device_malloc(&emb_data_, bytes, "cudaMalloc(embedding)");
             check(cudaMemcpy(emb_data_, data, bytes, cudaMemcpyHostToDevice), "upload embedding");
             emb_src_ = kind == KERNRT_F32 ? SRC_F32 : SRC_BF16;
         } else {
-            check(cudaMalloc(&emb_data_, n), "cudaMalloc(embedding)");
-            check(cudaMalloc(&emb_scales_, (n / 32) * sizeof(float)), "cudaMalloc(embedding scales)");
+            device_malloc(&emb_data_, n, "cudaMalloc(embedding)");
+            device_malloc(&emb_scales_, (n / 32) * sizeof(float), "cudaMalloc(embedding scales)");
             if (kind == KERNRT_Q8_0) {
                 check(cudaMemcpy(emb_data_, data, n, cudaMemcpyHostToDevice), "upload embedding");
                 check(cudaMemcpy(emb_scales_, scales, (n / 32) * sizeof(float), cudaMemcpyHostToDevice),
@@ -167,7 +167,7 @@ public:
                 // de-interleaved here to the row-major Q8_0 the kernels read.
                 const size_t blk_bytes = (vocab / 4) * (dim / 32) * 136;
                 void *tmp = nullptr;
-                check(cudaMalloc(&tmp, blk_bytes), "cudaMalloc(q8_0x4 staging)");
+                device_malloc(&tmp, blk_bytes, "cudaMalloc(q8_0x4 staging)");
                 cudaError_t e = cudaMemcpy(tmp, data, blk_bytes, cudaMemcpyHostToDevice);
                 if (e == cudaSuccess)
                     e = launch_q8x4_to_row_major(static_cast<const uint8_t *>(tmp), (int)vocab, (int)dim,
@@ -223,7 +223,7 @@ public:
             void *p = nullptr;
             ~Dev() { cudaFree(p); }
         } payload, wide, table, scales, scales16;
-        check(cudaMalloc(&payload.p, std::max<size_t>(t.end - t.start, 16)), "cudaMalloc(file payload)");
+        device_malloc(&payload.p, std::max<size_t>(t.end - t.start, 16), "cudaMalloc(file payload)");
         read_file(path, h.data_offset + t.start, t.end - t.start, payload.p);
         // f32 values of the table, where the route needs them
         const float *f = nullptr;
@@ -231,7 +231,7 @@ public:
             if (t.dtype == ST_F32) {
                 f = static_cast<const float *>(payload.p);
             } else {
-                check(cudaMalloc(&wide.p, n * sizeof(float)), "cudaMalloc(widened table)");
+                device_malloc(&wide.p, n * sizeof(float), "cudaMalloc(widened table)");
                 check(launch_widen_f32(t.dtype == ST_BF16 ? 1 : 2, static_cast<const uint16_t *>(payload.p),
                                        static_cast<float *>(wide.p), n, stream_),
                       "widen table");
@@ -250,14 +250,14 @@ public:
             kind = KERNRT_F32, src = SRC_F32;
             break;
         case TO_BF16:
-            check(cudaMalloc(&table.p, n * 2), "cudaMalloc(embedding)");
+            device_malloc(&table.p, n * 2, "cudaMalloc(embedding)");
             check(launch_narrow_bf16(f, static_cast<uint16_t *>(table.p), n, stream_), "narrow table");
             kind = KERNRT_BF16, src = SRC_BF16;
             break;
         default:  // TO_Q8, TO_Q8X4: Q8Vec::quantize's blocks (quant.rs:544-557, 124-165)
-            check(cudaMalloc(&table.p, n), "cudaMalloc(embedding)");
-            check(cudaMalloc(&scales.p, nb * sizeof(float)), "cudaMalloc(embedding scales)");
-            check(cudaMalloc(&scales16.p, nb * sizeof(uint16_t)), "cudaMalloc(f16 scales)");
+            device_malloc(&table.p, n, "cudaMalloc(embedding)");
+            device_malloc(&scales.p, nb * sizeof(float), "cudaMalloc(embedding scales)");
+            device_malloc(&scales16.p, nb * sizeof(uint16_t), "cudaMalloc(f16 scales)");
             check(launch_quantize_q8(f, (int)vocab, (int)dim, static_cast<int8_t *>(table.p),
                                      static_cast<float *>(scales.p), static_cast<uint16_t *>(scales16.p), stream_),
                   "quantize table");
@@ -445,15 +445,36 @@ public:
                 return p;
             }
         void *p = nullptr;
-        cudaError_t e = cudaMalloc(&p, size);
+        device_malloc(&p, size, what);
+        return p;
+    }
+    // Device memory for whatever the context makes: where the device has none left,
+    // the kept blocks go back to it first.
+    // Fault injection for tests: KERNRT_CUDA_FAIL_MALLOC=n makes the n-th of these
+    // calls find the device exhausted the first time it asks.
+    template <class T>
+    void device_malloc(T **p, size_t bytes, const char *what) {
+        cudaError_t e = ++mallocs_ == fail_malloc_at_ ? cudaErrorMemoryAllocation
+                                                      : cudaMalloc(reinterpret_cast<void **>(p), bytes);
         if (e == cudaErrorMemoryAllocation && !spare_.empty()) {
             cudaGetLastError();
             drop_spare(0);
-            e = cudaMalloc(&p, size);
+            e = cudaMalloc(reinterpret_cast<void **>(p), bytes);
         }
         if (e != cudaSuccess) cudaGetLastError();
         check(e, what);
-        return p;
+    }
+    // The same in the order of the stream (inside a capture nothing is given back).
+    template <class T>
+    void stream_malloc(T **p, size_t bytes, const char *what) {
+        cudaError_t e = cudaMallocAsync(reinterpret_cast<void **>(p), bytes, stream_);
+        if (e == cudaErrorMemoryAllocation && !spare_.empty() && !capturing()) {
+            cudaGetLastError();
+            drop_spare(0);
+            e = cudaMallocAsync(reinterpret_cast<void **>(p), bytes, stream_);
+        }
+        if (e != cudaSuccess) cudaGetLastError();
+        check(e, what);
     }
     void give_block(void *p, size_t bytes) {
         if (!p) return;
@@ -541,12 +562,12 @@ public:
         try {
             if (kind == KERNRT_F32 || kind == KERNRT_BF16) {
                 const size_t bytes = n * (kind == KERNRT_F32 ? 4 : 2);
-                check(cudaMalloc(&m.data, bytes), "cudaMalloc(matrix)");
+                device_malloc(&m.data, bytes, "cudaMalloc(matrix)");
                 check(cudaMemcpy(m.data, data, bytes, cudaMemcpyHostToDevice), "upload matrix");
                 m.src = kind == KERNRT_F32 ? SRC_F32 : SRC_BF16;
             } else {
-                check(cudaMalloc(&m.data, n), "cudaMalloc(matrix)");
-                check(cudaMalloc(&m.scales, (n / 32) * sizeof(float)), "cudaMalloc(matrix scales)");
+                device_malloc(&m.data, n, "cudaMalloc(matrix)");
+                device_malloc(&m.scales, (n / 32) * sizeof(float), "cudaMalloc(matrix scales)");
                 if (kind == KERNRT_Q8_0) {
                     check(cudaMemcpy(m.data, data, n, cudaMemcpyHostToDevice), "upload matrix");
                     check(cudaMemcpy(m.scales, scales, (n / 32) * sizeof(float), cudaMemcpyHostToDevice),
@@ -554,7 +575,7 @@ public:
                 } else {
                     const size_t blk_bytes = (out_dim / 4) * (in_dim / 32) * 136;
                     void *tmp = nullptr;
-                    check(cudaMalloc(&tmp, blk_bytes), "cudaMalloc(q8_0x4 staging)");
+                    device_malloc(&tmp, blk_bytes, "cudaMalloc(q8_0x4 staging)");
                     cudaError_t e = cudaMemcpy(tmp, data, blk_bytes, cudaMemcpyHostToDevice);
                     if (e == cudaSuccess)
                         e = launch_q8x4_to_row_major(static_cast<const uint8_t *>(tmp), (int)out_dim, (int)in_dim,
@@ -599,13 +620,17 @@ public:
             cudaFree(split_);
             split_ = nullptr;
             split_cap_ = 0;
-            check(cudaMalloc(&split_, 2 * n * sizeof(uint16_t)), "cudaMalloc(split activations)");
+            device_malloc(&split_, 2 * n * sizeof(uint16_t), "cudaMalloc(split activations)");
             split_cap_ = 2 * n;
         }
         launch_or_fail(launch_split_bf16(x, split_, split_ + n, n, stream_), "project (split)");
         return split_;
     }
     void set_fail_alloc(uint64_t n) { fail_alloc_at_ = n; }
+    void set_fail_malloc(uint64_t n) {  // counted from here
+        mallocs_ = 0;
+        fail_malloc_at_ = n;
+    }
     void set_exact(bool exact) {
         flush();
         exact_ = exact;
@@ -714,8 +739,8 @@ public:
         cudaFree(vc_);
         kc_ = vc_ = nullptr;
         const size_t bytes = n_layers * seq_len * kv_dim * sizeof(float);
-        check(cudaMalloc(&kc_, bytes), "cudaMalloc(key cache)");
-        check(cudaMalloc(&vc_, bytes), "cudaMalloc(value cache)");
+        device_malloc(&kc_, bytes, "cudaMalloc(key cache)");
+        device_malloc(&vc_, bytes, "cudaMalloc(value cache)");
         check(cudaMemsetAsync(kc_, 0, bytes, stream_), "cudaMemset");
         check(cudaMemsetAsync(vc_, 0, bytes, stream_), "cudaMemset");
         kv_layers_ = n_layers;
@@ -817,7 +842,7 @@ public:
             cudaFree(att_scratch_);
             att_scratch_ = nullptr;
             att_scratch_bytes_ = 0;
-            check(cudaMalloc(&att_scratch_, need), "cudaMalloc(attention scratch)");
+            device_malloc(&att_scratch_, need, "cudaMalloc(attention scratch)");
             att_scratch_bytes_ = need;
         }
         // windows that differ only in their last slot map positions alike
@@ -850,7 +875,7 @@ public:
         if (src == dst && sp != dp && sp < dp + bytes && dp < sp + bytes) {
             // copy_within: overlapping ranges go through a temporary.
             void *tmp = nullptr;
-            check(cudaMallocAsync(&tmp, bytes, stream_), "cudaMallocAsync");
+            stream_malloc(&tmp, bytes, "cudaMallocAsync");
             check(cudaMemcpyAsync(tmp, sp, bytes, cudaMemcpyDeviceToDevice, stream_), "copy");
             check(cudaMemcpyAsync(dp, tmp, bytes, cudaMemcpyDeviceToDevice, stream_), "copy");
             check(cudaFreeAsync(tmp, stream_), "cudaFreeAsync");
@@ -1035,12 +1060,12 @@ public:
         const float *xp = f(xb), *kp = f(kb);
         void *tx = nullptr, *tk = nullptr;
         if (x == out) {
-            check(cudaMallocAsync(&tx, rows * dim * 4, stream_), "cudaMallocAsync");
+            stream_malloc(&tx, rows * dim * 4, "cudaMallocAsync");
             check(cudaMemcpyAsync(tx, xp, rows * dim * 4, cudaMemcpyDeviceToDevice, stream_), "copy");
             xp = static_cast<const float *>(tx);
         }
         if (kernel == out) {
-            check(cudaMallocAsync(&tk, dim * k * 4, stream_), "cudaMallocAsync");
+            stream_malloc(&tk, dim * k * 4, "cudaMallocAsync");
             check(cudaMemcpyAsync(tk, kp, dim * k * 4, cudaMemcpyDeviceToDevice, stream_), "copy");
             kp = static_cast<const float *>(tk);
         }
@@ -1290,7 +1315,7 @@ public:
                 cudaFree(set.arena);
                 set.arena = nullptr;
                 set.bytes = 0;
-                check(cudaMalloc(&set.arena, arena), "cudaMalloc(host pipeline)");
+                device_malloc(&set.arena, arena, "cudaMalloc(host pipeline)");
                 set.bytes = arena;
             }
             set.used = false;
@@ -2041,7 +2066,7 @@ private:
             cudaFree(row_scales_);
             row_scales_ = nullptr;
             row_scales_cap_ = 0;
-            check(cudaMalloc(&row_scales_, rows * sizeof(float)), "cudaMalloc(row scales)");
+            device_malloc(&row_scales_, rows * sizeof(float), "cudaMalloc(row scales)");
             row_scales_cap_ = rows;
         }
         return row_scales_;
@@ -2101,8 +2126,8 @@ private:
         if (t->sin) check(cudaFreeAsync(t->sin, stream_), "cudaFreeAsync(rope)");
         t->cos = t->sin = nullptr;
         t->max_pos = 0;
-        check(cudaMallocAsync(reinterpret_cast<void **>(&t->cos), n * 4, stream_), "cudaMallocAsync(rope)");
-        check(cudaMallocAsync(reinterpret_cast<void **>(&t->sin), n * 4, stream_), "cudaMallocAsync(rope)");
+        stream_malloc(&t->cos, n * 4, "cudaMallocAsync(rope)");
+        stream_malloc(&t->sin, n * 4, "cudaMallocAsync(rope)");
         check(cudaMemcpyAsync(t->cos, hc.data(), n * 4, cudaMemcpyHostToDevice, stream_), "upload rope table");
         check(cudaMemcpyAsync(t->sin, hs.data(), n * 4, cudaMemcpyHostToDevice, stream_), "upload rope table");
         t->max_pos = cap;
@@ -2165,7 +2190,7 @@ private:
         stage_host_ = nullptr;
         stage_dev_ = nullptr;
         check(cudaHostAlloc(&stage_host_, cap, cudaHostAllocMapped), "cudaHostAlloc(staging)");
-        check(cudaMalloc(&stage_dev_, cap), "cudaMalloc(staging)");
+        device_malloc(&stage_dev_, cap, "cudaMalloc(staging)");
         void *map = nullptr;
         stage_map_ = nullptr;
         if (cudaHostGetDevicePointer(&map, stage_host_, 0) == cudaSuccess) stage_map_ = static_cast<char *>(map);
@@ -2275,6 +2300,8 @@ private:
     bool exact_ = true;             // false: tolerance-mode tensor-core projections (KERNRT_CUDA_EXACT=0)
     uint64_t allocs_ = 0;           // buffer allocations so far
     uint64_t fail_alloc_at_ = 0;    // the allocation to fail (KERNRT_CUDA_FAIL_ALLOC; 0 = none)
+    uint64_t mallocs_ = 0;          // requests for device memory so far
+    uint64_t fail_malloc_at_ = 0;   // the one that finds none (KERNRT_CUDA_FAIL_MALLOC; 0 = none)
     uint16_t *split_ = nullptr;     // bf16 hi / lo halves of a projection's x
     size_t split_cap_ = 0;          // elements
     float *row_scales_ = nullptr;   // the two-pass norm stage's row scales (chains on stream_)
@@ -2422,6 +2449,9 @@ int kernrt_cuda_create(int device, kernrt_cuda_ctx **out) {
         // test hook, off unless set: fail this context's n-th buffer allocation
         const char *fail_at = std::getenv("KERNRT_CUDA_FAIL_ALLOC");
         if (fail_at && *fail_at) c->b->set_fail_alloc(std::strtoull(fail_at, nullptr, 10));
+        // and another: its n-th request for device memory finds none
+        const char *none_at = std::getenv("KERNRT_CUDA_FAIL_MALLOC");
+        if (none_at && *none_at) c->b->set_fail_malloc(std::strtoull(none_at, nullptr, 10));
         *out = c;
         return KERNRT_OK;
     } catch (const krt::Error &e) {

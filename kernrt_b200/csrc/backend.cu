@@ -149,6 +149,7 @@ public:
         cudaFree(emb_scales_);
         emb_data_ = nullptr;
         emb_scales_ = nullptr;
+        emb_kind_ = -1;  // none, until this one is there
         const size_t n = vocab * dim;
         if (kind == KERNRT_F32 || kind == KERNRT_BF16) {
             const size_t bytes = n * (kind == KERNRT_F32 ? 4 : 2);
@@ -739,8 +740,15 @@ public:
         cudaFree(vc_);
         kc_ = vc_ = nullptr;
         const size_t bytes = n_layers * seq_len * kv_dim * sizeof(float);
-        device_malloc(&kc_, bytes, "cudaMalloc(key cache)");
-        device_malloc(&vc_, bytes, "cudaMalloc(value cache)");
+        float *kc = nullptr;
+        device_malloc(&kc, bytes, "cudaMalloc(key cache)");
+        try {
+            device_malloc(&vc_, bytes, "cudaMalloc(value cache)");
+        } catch (...) {
+            cudaFree(kc);
+            throw;
+        }
+        kc_ = kc;  // (there is a cache where both are)
         check(cudaMemsetAsync(kc_, 0, bytes, stream_), "cudaMemset");
         check(cudaMemsetAsync(vc_, 0, bytes, stream_), "cudaMemset");
         kv_layers_ = n_layers;

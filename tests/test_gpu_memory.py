@@ -48,3 +48,53 @@ def test_kept_blocks_go_back_before_a_call_fails(name):
         assert e.value.code == kernrt_b200.E_CUDA and "memory" in str(e.value)
         CALLS[name](b)  # there is some again
         b.synchronize()
+
+
+@pytest.mark.parametrize("part", [0, 1], ids=["keys", "values"])
+def test_a_key_value_cache_whose_allocation_fails_is_not_there(part):
+    """Nor the one before it, whose memory is gone."""
+    rows = np.random.default_rng(1).standard_normal((3, 64)).astype(np.float32)
+    with context(4 + part) as b:
+        hk, hv = b.upload(rows), b.upload(-rows)  # requests 1 and 2
+        hs = hk, hv, b.alloc(3 * 64)              # 3
+        q, out, att = hs[0], hs[2], None
+        with pytest.raises(KernrtCudaError) as e:
+            b.kv_prepare(1, 64, 8)
+        assert e.value.code == kernrt_b200.E_CUDA
+        att = b.alloc(3 * 8)
+
+        def write():
+            b.kv_write(0, [0, 1, 2], hk, hv, 3)
+
+        def attend():
+            b.attention(q, out, att, 0, [(0, i, 0, 0) for i in range(3)], 1, 1, 64, 64, 8)
+
+        for call in (write, attend):
+            with pytest.raises(KernrtCudaError) as e:
+                call()
+            assert e.value.code == kernrt_b200.E_STATE
+        b.kv_prepare(1, 64, 8)
+        write()
+        attend()
+        assert np.array_equal(b.read(out, 64), -rows[0])  # one key: its value
+
+
+@pytest.mark.parametrize("part", [0, 1], ids=["codes", "scales"])
+def test_an_embedding_whose_allocation_fails_is_not_there(part):
+    """Nor the one before it, whose memory is gone."""
+    table = np.random.default_rng(2).standard_normal((8, 32)).astype(np.float32)
+    codes, scales = np.arange(8 * 32, dtype=np.int8), np.ones(8, np.float32)
+    with context(3 + part) as b:
+        x = b.alloc(32)                                     # request 1
+        b.prepare_embedding(F32, table, None, 8, 32)        # 2
+        b.embed(5, x, 0)
+        assert np.array_equal(b.read(x, 32), table[5])
+        with pytest.raises(KernrtCudaError) as e:
+            b.prepare_embedding(kernrt_b200.Q8_0, codes, scales, 8, 32)
+        assert e.value.code == kernrt_b200.E_CUDA
+        with pytest.raises(KernrtCudaError) as e:
+            b.embed(5, x, 0)
+        assert e.value.code == kernrt_b200.E_STATE
+        b.prepare_embedding(kernrt_b200.Q8_0, codes, scales, 8, 32)
+        b.embed(5, x, 0)
+        assert np.array_equal(b.read(x, 32), codes.reshape(8, 32)[5].astype(np.float32))

@@ -2194,11 +2194,18 @@ private:
     }
 
     void grow_staging(size_t cap) {
-        if (stage_host_ || stage_dev_) retired_.push_back({stage_host_, stage_dev_});
-        stage_host_ = nullptr;
-        stage_dev_ = nullptr;
-        check(cudaHostAlloc(&stage_host_, cap, cudaHostAllocMapped), "cudaHostAlloc(staging)");
-        device_malloc(&stage_dev_, cap, "cudaMalloc(staging)");
+        char *host = nullptr, *dev = nullptr;  // both, or the old ring stays
+        check(cudaHostAlloc(&host, cap, cudaHostAllocMapped), "cudaHostAlloc(staging)");
+        try {
+            device_malloc(&dev, cap, "cudaMalloc(staging)");
+            if (stage_host_) retired_.push_back({stage_host_, stage_dev_});
+        } catch (...) {
+            cudaFreeHost(host);
+            cudaFree(dev);
+            throw;
+        }
+        stage_host_ = host;
+        stage_dev_ = dev;
         void *map = nullptr;
         stage_map_ = nullptr;
         if (cudaHostGetDevicePointer(&map, stage_host_, 0) == cudaSuccess) stage_map_ = static_cast<char *>(map);

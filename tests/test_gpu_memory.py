@@ -98,3 +98,24 @@ def test_an_embedding_whose_allocation_fails_is_not_there(part):
         b.prepare_embedding(kernrt_b200.Q8_0, codes, scales, 8, 32)
         b.embed(5, x, 0)
         assert np.array_equal(b.read(x, 32), codes.reshape(8, 32)[5].astype(np.float32))
+
+
+def test_staging_that_cannot_grow_stays_as_it_was():
+    """More rows' tokens in one call than the staging ring takes: it grows; a call
+    that finds no memory for that fails, and smaller ones go on as before."""
+    rows, dim, seq = 60000, 4, 60000
+    k = np.random.default_rng(3).standard_normal((rows, dim)).astype(np.float32)
+    with context(6) as b:
+        hk, hv = b.upload(k), b.upload(-k)     # requests 1 and 2
+        out = b.alloc(dim)                      # 3
+        b.kv_prepare(1, dim, seq)               # 4 and 5
+        with pytest.raises(KernrtCudaError) as e:
+            b.kv_write(0, np.arange(rows), hk, hv, rows)
+        assert e.value.code == kernrt_b200.E_CUDA
+        att = b.alloc(seq)
+        for n in (3, 1000, rows):
+            for _ in range(20):  # around the ring
+                b.kv_write(0, np.arange(rows - n, rows), hk, hv, n)
+                b.synchronize()
+            b.attention(hk, out, att, 0, [(rows - n, rows - n, 0, 0)], 1, 1, dim, dim, seq)
+            assert np.array_equal(b.read(out, dim), -k[0])

@@ -411,7 +411,8 @@ int kernrt_cuda_attention(kernrt_cuda_ctx *ctx, kernrt_buf q, kernrt_buf out, ke
  *
  * Failures of the bookkeeping change nothing: KERNRT_E_STATE when the pool has
  * too few pages or sequences left, KERNRT_E_INVALID for bad arguments (a closed
- * sequence, one named twice in a call, a length past max_len). */
+ * sequence, one named twice in a call, a length past max_len).  Nor does a step, a
+ * copy or a compaction whose device work cannot be enqueued (KERNRT_E_CUDA). */
 typedef uint64_t kernrt_pages;
 
 /* A cache for at most max_seqs sequences of at most max_len positions over a

@@ -1581,8 +1581,13 @@ public:
         flush();
         std::vector<PageCopy> copies;
         const uint64_t got = paging([&] { return c.map->copy(seq, length, &copies); });
+        try {
+            copy_pages(c, copies);
+        } catch (...) {
+            c.map->close(&got, 1);
+            throw;
+        }
         c.stepped = false;
-        copy_pages(c, copies);
         return got;
     }
 
@@ -1603,9 +1608,10 @@ public:
         PagedCache &c = cache(h);
         not_captured("pages_compact");
         flush();
-        const std::vector<PageCopy> moves = c.map->compact();
+        const std::vector<PageCopy> moves = c.map->plan_compact();
+        copy_pages(c, moves);  // (into free pages: the tables follow)
+        c.map->make_compact(moves);
         if (!moves.empty()) c.stepped = false;
-        copy_pages(c, moves);
         return moves.size();
     }
 
@@ -1769,8 +1775,24 @@ public:
         flush();
         std::vector<PageCopy> copies;
         paging([&] { c.map->extend(seqs, rows, n, &copies); });
-        c.stepped = false;
         std::vector<StepSeq> desc;
+        size_t row0 = 0;
+        try {
+            row0 = bring_step(c, seqs, rows, n, copies, &desc);
+        } catch (...) {  // nothing reached the device: the last step stands
+            c.map->undo_extend(seqs, rows, n, std::move(copies));
+            throw;
+        }
+        for (const StepSeq &q : desc) c.map->at((size_t)q.slot).dirty = c.map->at((size_t)q.slot).pages.size();
+        c.rows = row0;
+        c.step = std::move(desc);
+        c.planned = false;
+        c.stepped = true;
+    }
+    // The step's descriptors, and all of it to the device in one upload: the
+    // descriptors, the tables' changes, the copies of shared pages.
+    size_t bring_step(PagedCache &c, const uint64_t *seqs, const uint64_t *rows, size_t n,
+                      const std::vector<PageCopy> &copies, std::vector<StepSeq> *desc) {
         std::vector<int32_t> delta;
         size_t row0 = 0;
         for (size_t i = 0; i < n; ++i) {
@@ -1786,28 +1808,20 @@ public:
             d.n_dirty = (int32_t)(q.pages.size() - q.dirty);
             d.delta = (int32_t)delta.size();
             delta.insert(delta.end(), q.pages.begin() + (long)q.dirty, q.pages.end());
-            desc.push_back(d);
+            desc->push_back(d);
             row0 += (size_t)rows[i];
         }
-        c.rows = row0;
-        c.planned = false;
-        if (!desc.empty()) {
-            // one upload: the descriptors, the tables' changes, the copies of
-            // shared pages
-            const size_t a = desc.size() * sizeof(StepSeq), b = delta.size() * sizeof(int32_t);
-            std::vector<char> block(a + b + copies.size() * sizeof(CopyItem));
-            std::memcpy(block.data(), desc.data(), a);
-            if (b) std::memcpy(block.data() + a, delta.data(), b);
-            if (!copies.empty()) std::memcpy(block.data() + a + b, copies.data(), copies.size() * sizeof(CopyItem));
-            const char *d = static_cast<const char *>(stage(block.data(), block.size()));
-            launch_or_fail(launch_pages_step(c.view, reinterpret_cast<const StepSeq *>(d), (int)desc.size(), c.seqs,
-                                             c.table, reinterpret_cast<const CopyItem *>(d + a + b),
-                                             (int)copies.size(), stream_),
-                           "pages_step");
-            for (const StepSeq &q : desc) c.map->at((size_t)q.slot).dirty = c.map->at((size_t)q.slot).pages.size();
-        }
-        c.step = std::move(desc);
-        c.stepped = true;
+        if (desc->empty()) return 0;
+        const size_t a = desc->size() * sizeof(StepSeq), b = delta.size() * sizeof(int32_t);
+        std::vector<char> block(a + b + copies.size() * sizeof(CopyItem));
+        std::memcpy(block.data(), desc->data(), a);
+        if (b) std::memcpy(block.data() + a, delta.data(), b);
+        if (!copies.empty()) std::memcpy(block.data() + a + b, copies.data(), copies.size() * sizeof(CopyItem));
+        const char *d = static_cast<const char *>(stage(block.data(), block.size()));
+        launch_or_fail(launch_pages_step(c.view, reinterpret_cast<const StepSeq *>(d), (int)desc->size(), c.seqs, c.table,
+                                         reinterpret_cast<const CopyItem *>(d + a + b), (int)copies.size(), stream_),
+                       "pages_step");
+        return row0;
     }
 
     PagedCache &stepped_cache(uint64_t h, size_t layer) {

@@ -172,21 +172,48 @@ void PageMap::extend(const uint64_t *seqs, const uint64_t *rows, size_t n, std::
     }
 }
 
-std::vector<PageCopy> PageMap::compact() {
+void PageMap::undo_extend(const uint64_t *seqs, const uint64_t *rows, size_t n, std::vector<PageCopy> copies) {
+    for (size_t i = n; i-- > 0;) {
+        if (rows[i] == 0) continue;
+        Seq &q = seqs_[slot(seqs[i])];
+        q.len -= (size_t)rows[i];
+        while (q.pages.size() > pages_for(q.len)) {
+            release(q.pages.back());
+            q.pages.pop_back();
+        }
+        // the copies are in the order of the sequences that took them
+        if (!copies.empty() && q.len % page_size_ != 0 && copies.back().dst == q.pages.back()) {
+            release(q.pages.back());
+            q.pages.back() = copies.back().src;
+            ++refs_[(size_t)copies.back().src];
+            copies.pop_back();
+        }
+        q.dirty = std::min(q.dirty, q.pages.size());
+    }
+}
+
+std::vector<PageCopy> PageMap::plan_compact() const {
     const size_t used = refs_.size() - free_.size();
     std::vector<PageCopy> moves;
-    std::vector<int32_t> to(refs_.size());
-    for (size_t i = 0; i < to.size(); ++i) to[i] = (int32_t)i;
     size_t hole = 0;
     for (size_t p = refs_.size(); p-- > used;) {
         if (refs_[p] == 0) continue;
         while (refs_[hole] != 0) ++hole;
-        to[p] = (int32_t)hole;
-        refs_[hole] = refs_[p];
-        refs_[p] = 0;
-        moves.push_back({(int32_t)p, (int32_t)hole, (int32_t)page_size_});
+        moves.push_back({(int32_t)p, (int32_t)hole++, (int32_t)page_size_});
     }
-    if (moves.empty()) return moves;
+    return moves;
+}
+
+void PageMap::make_compact(const std::vector<PageCopy> &moves) {
+    if (moves.empty()) return;
+    const size_t used = refs_.size() - free_.size();
+    std::vector<int32_t> to(refs_.size());
+    for (size_t i = 0; i < to.size(); ++i) to[i] = (int32_t)i;
+    for (const PageCopy &m : moves) {
+        to[(size_t)m.src] = m.dst;
+        refs_[(size_t)m.dst] = refs_[(size_t)m.src];
+        refs_[(size_t)m.src] = 0;
+    }
     for (Seq &q : seqs_) {
         if (!q.open) continue;
         for (size_t i = 0; i < q.pages.size(); ++i) {
@@ -198,7 +225,6 @@ std::vector<PageCopy> PageMap::compact() {
     }
     free_.clear();
     for (size_t p = used; p < refs_.size(); ++p) free_.push_back((int32_t)p);
-    return moves;
 }
 
 }  // namespace krt

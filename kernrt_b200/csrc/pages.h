@@ -1,7 +1,9 @@
 // Host bookkeeping of a paged key/value cache: which pages each sequence
 // holds, how many sequences share a page, and which pages are free.  No device
 // calls: every operation that moves cache contents returns the page copies the
-// caller has to enqueue.  A failing call throws PageError and changes nothing.
+// caller has to enqueue.  A failing call throws PageError and changes nothing; a
+// caller that cannot enqueue the copies takes the operation back (undo_extend;
+// close for copy; compaction is planned first and made after).
 //
 // Pages are taken lowest id first.  A page several sequences share is never
 // written: a sequence that grows into its last, partly filled page while others
@@ -47,9 +49,17 @@ public:
     void close(const uint64_t *seqs, size_t n);
     // Every sequence seqs[i] grows by rows[i] positions.
     void extend(const uint64_t *seqs, const uint64_t *rows, size_t n, std::vector<PageCopy> *copies);
+    // Takes the last call back, an extend with these sequences, rows and copies.
+    void undo_extend(const uint64_t *seqs, const uint64_t *rows, size_t n, std::vector<PageCopy> copies);
     // Moves the highest pages in use into the lowest free ones until the pages
     // in use are 0 .. count - 1; returns the moves.
-    std::vector<PageCopy> compact();
+    std::vector<PageCopy> compact() {
+        std::vector<PageCopy> moves = plan_compact();
+        make_compact(moves);
+        return moves;
+    }
+    std::vector<PageCopy> plan_compact() const;        // the moves, nothing changed
+    void make_compact(const std::vector<PageCopy> &);  // as planned, nothing between
 
     size_t slot(uint64_t seq) const;  // throws on a closed or unknown handle
     Seq &at(size_t slot) { return seqs_[slot]; }

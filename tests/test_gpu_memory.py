@@ -119,3 +119,107 @@ def test_staging_that_cannot_grow_stays_as_it_was():
                 b.synchronize()
             b.attention(hk, out, att, 0, [(rows - n, rows - n, 0, 0)], 1, 1, dim, dim, seq)
             assert np.array_equal(b.read(out, dim), -k[0])
+
+
+def pages(b, n_pages, max_seqs, page=16, max_len=400000):
+    from kernrt_b200.interop import pages_as_torch
+
+    p = b.pages_create(F32, 1, 1, 1, 8, page, n_pages, max_seqs, max_len)  # requests 1 to 3
+    b.synchronize()
+    return p, pages_as_torch(b, p)[0, :, :, 0]  # [K or V, page, position, 8]
+
+
+def write(b, p, rows, start):
+    """Rows start, start + 1 .. of K (and their negatives of V) into the step."""
+    k = np.repeat(np.arange(start, start + rows, dtype=np.float32), 8)
+    hk, hv = b.upload(k), b.upload(-k)
+    b.pages_write(p, 0, hk, hv)
+    b.synchronize()
+
+
+def content(view, table, length):
+    k, v = view[:, table.tolist()].reshape(2, -1, 8)[:, :length].cpu().numpy()
+    assert np.array_equal(k, -v) and (k == k[:, :1]).all()
+    return k[:, 0].astype(int).tolist()
+
+
+def fails(call):
+    with pytest.raises(KernrtCudaError) as e:
+        call()
+    assert e.value.code == kernrt_b200.E_CUDA and "staging" in str(e.value)
+
+
+def test_a_step_that_cannot_be_enqueued_changes_nothing():
+    """4,000 forks of five positions take a copy each of their shared page: more than
+    a segment of the staging ring, which finds no memory to grow."""
+    n = 4000
+    with context(6) as b:
+        p, view = pages(b, n + 10, n + 2)
+        s = b.seq_open(p)
+        b.pages_step(p, [s], [5])
+        write(b, p, 5, 100)  # requests 4 and 5
+        kids = b.seq_fork(p, s, 5, n)
+        free, table = b.pages_ptr(p).available, b.seq_table(p, s).tolist()
+        fails(lambda: b.pages_step(p, kids, [1] * n))
+        assert b.pages_ptr(p).available == free
+        for q in [s, kids[0], kids[1], kids[-1]]:
+            assert b.seq_length(p, q) == 5 and b.seq_table(p, q).tolist() == table
+        b.pages_step(p, kids, [1] * n)  # there is memory again
+        write(b, p, n, 1000)
+        for i in (0, 1, 777, n - 1):
+            assert content(view, b.seq_table(p, kids[i]), 6) == [100, 101, 102, 103, 104, 1000 + i]
+        assert content(view, b.seq_table(p, s), 5) == [100, 101, 102, 103, 104]
+        assert len({int(b.seq_table(p, q)[0]) for q in kids + [s]}) == n + 1
+
+
+def test_a_step_that_cannot_be_enqueued_leaves_the_one_before_it():
+    n = 4000
+    with context(6) as b:
+        p, view = pages(b, n + 10, n + 2)
+        s, t = b.seq_open(p), b.seq_open(p)
+        b.pages_step(p, [s], [5])
+        write(b, p, 5, 100)  # requests 4 and 5
+        kids = b.seq_fork(p, s, 5, n)
+        b.pages_step(p, [t], [3])
+        fails(lambda: b.pages_step(p, kids, [1] * n))
+        write(b, p, 3, 7)  # t's rows
+        assert content(view, b.seq_table(p, t), 3) == [7, 8, 9]
+        assert content(view, b.seq_table(p, kids[5]), 5) == [100, 101, 102, 103, 104]
+
+
+def test_a_copy_that_cannot_be_enqueued_opens_no_sequence():
+    length = 16 * 11000 + 3  # as many page copies do not fit the ring
+    with context(6) as b:
+        p, view = pages(b, 22010, 3)
+        s = b.seq_open(p)
+        b.pages_step(p, [s], [length])
+        write(b, p, length, 0)  # requests 4 and 5
+        free = b.pages_ptr(p).available
+        fails(lambda: b.seq_copy(p, s, length))
+        assert b.pages_ptr(p).available == free
+        write(b, p, length, 1)  # the step stands
+        others = [b.seq_copy(p, s, length), b.seq_open(p)]  # both places are free
+        b.synchronize()
+        assert content(view, b.seq_table(p, others[0]), length) == list(range(1, length + 1))
+        with pytest.raises(KernrtCudaError):
+            b.seq_open(p)
+
+
+def test_a_compaction_that_cannot_be_enqueued_moves_nothing():
+    length = 16 * 11000 + 3
+    with context(6) as b:
+        p, view = pages(b, 22010, 3)
+        gone, s = b.seq_open(p), b.seq_open(p)
+        b.pages_step(p, [gone, s], [length, 3])
+        b.seq_close(p, [])
+        b.pages_step(p, [s], [length - 3])
+        write(b, p, length - 3, 3)  # requests 4 and 5
+        b.seq_close(p, [gone])
+        free, table = b.pages_ptr(p).available, b.seq_table(p, s).tolist()
+        fails(lambda: b.pages_compact(p))
+        assert b.pages_ptr(p).available == free and b.seq_table(p, s).tolist() == table
+        assert content(view, b.seq_table(p, s), length)[3:] == list(range(3, length))
+        assert b.pages_compact(p) == 11001
+        b.synchronize()
+        assert sorted(b.seq_table(p, s).tolist()) == list(range(11001))
+        assert content(view, b.seq_table(p, s), length)[3:] == list(range(3, length))

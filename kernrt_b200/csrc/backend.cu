@@ -1501,15 +1501,17 @@ public:
         const size_t big = (size_t)INT32_MAX;
         if (n_layers > 65535 || n_heads > 65535 || max_seqs > 65535 || n_pages > big / 4 || max_len > big / 4)
             fail(KERNRT_E_INVALID, "page cache too large");
-        // rows of head_size elements, addressed by a signed 32-bit coordinate
-        if (n_layers * 2 * n_kv_heads * page_size > big / n_pages) fail(KERNRT_E_INVALID, "page cache too large");
+        // 256 GB, more than the device has (addresses are 64-bit; pages x layers x kv
+        // heads stay within 32)
+        const size_t page_bytes = n_layers * 2 * n_kv_heads * page_size * head_size * (kind == KERNRT_F32 ? 4 : 2);
+        if (page_bytes > ((size_t)1 << 38) / n_pages) fail(KERNRT_E_INVALID, "page cache too large");
         const size_t max_pages = (max_len + page_size - 1) / page_size;
         if (max_pages > big / max_seqs) fail(KERNRT_E_INVALID, "page tables too large");
         not_captured("pages_create");
         flush();
         PagedCache c;
         c.map = std::make_unique<PageMap>(n_pages, page_size, max_seqs, max_len);
-        const size_t bytes = n_layers * 2 * n_pages * n_kv_heads * page_size * head_size * (kind == KERNRT_F32 ? 4 : 2);
+        const size_t bytes = n_pages * page_bytes;
         try {
             c.kv_bytes = bytes;
             c.table_bytes = max_seqs * max_pages * sizeof(int32_t);

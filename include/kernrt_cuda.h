@@ -137,8 +137,12 @@ int kernrt_cuda_device_ptr(kernrt_cuda_ctx *ctx, kernrt_buf buf, void **ptr);
  * goes; a serving process outlives its requests).  The handle is invalid from
  * then on and is not used again.  The context keeps freed memory, at most 8 GB
  * of it, for its next allocations, whose work is ordered behind the work already
- * enqueued; work of the caller's own on other streams has to be done. */
+ * enqueued; work of the caller's own on other streams has to be done.  Where one
+ * of its allocations finds the device exhausted, the kept memory goes back first. */
 int kernrt_cuda_free(kernrt_cuda_ctx *ctx, kernrt_buf buf);
+/* Gives the kept memory back to the device, for other allocators of the process
+ * and other processes; waits for the work that may still use it. */
+int kernrt_cuda_release_freed(kernrt_cuda_ctx *ctx);
 /* Wait for all deferred work. */
 int kernrt_cuda_synchronize(kernrt_cuda_ctx *ctx);
 /* Launch every deferred op (pending embeds, an op held for fusion) onto the
@@ -406,7 +410,7 @@ int kernrt_cuda_attention(kernrt_cuda_ctx *ctx, kernrt_buf q, kernrt_buf out, ke
  * valid for replays within that step only, one after the other (and the step's
  * first attention call, which lays its plan down, is made before the capture).
  * Calls that cannot be replayed (pages_create, _destroy, _step, _compact, seq_copy,
- * a step's first attention, kernrt_cuda_free) fail with KERNRT_E_STATE inside a
+ * a step's first attention, kernrt_cuda_free, _release_freed) fail with KERNRT_E_STATE inside a
  * capture of the context's stream and change nothing.
  *
  * Failures of the bookkeeping change nothing: KERNRT_E_STATE when the pool has

@@ -150,6 +150,7 @@ SIGNATURES = {
     "kernrt_cuda_selftest_wait": (C.c_int, [P, C.c_uint64, C.c_int]),
     "kernrt_cuda_set_exact": (C.c_int, [P, C.c_int]),
     "kernrt_cuda_free": (C.c_int, [P, Buf]),
+    "kernrt_cuda_release_freed": (C.c_int, [P]),
     "kernrt_cuda_pages_create": (C.c_int, [P, C.c_int, SZ, SZ, SZ, SZ, SZ, SZ, SZ, SZ, C.POINTER(C.c_uint64)]),
     "kernrt_cuda_pages_destroy": (C.c_int, [P, C.c_uint64]),
     "kernrt_cuda_pages_ptr": (C.c_int, [P, C.c_uint64, C.POINTER(PagesInfo)]),
@@ -350,6 +351,11 @@ class CudaBackend:
     def free(self, buf: int) -> None:
         """Gives the buffer's memory back; the handle is not used again."""
         _ok(self._lib.kernrt_cuda_free(self._ctx, buf))
+
+    def release_freed(self) -> None:
+        """Gives the memory that the context keeps of freed buffers and caches back
+        to the device (torch's allocator, say, does not know of it)."""
+        _ok(self._lib.kernrt_cuda_release_freed(self._ctx))
 
     def synchronize(self) -> None:
         _ok(self._lib.kernrt_cuda_synchronize(self._ctx))

@@ -492,6 +492,11 @@ public:
         spare_.erase(spare_.begin(), spare_.begin() + (long)n);
     }
 
+    void release_freed() {
+        not_captured("release_freed");
+        drop_spare(0);
+    }
+
     // Completes deferred work and surfaces device-reported input errors.
     void barrier() {
         flush();
@@ -2718,6 +2723,10 @@ int kernrt_cuda_attention(kernrt_cuda_ctx *ctx, kernrt_buf q, kernrt_buf out, ke
 
 int kernrt_cuda_free(kernrt_cuda_ctx *ctx, kernrt_buf buf) {
     return guard(ctx, [&](krt::Backend &b) { b.free_buf(buf); });
+}
+
+int kernrt_cuda_release_freed(kernrt_cuda_ctx *ctx) {
+    return guard(ctx, [&](krt::Backend &b) { b.release_freed(); });
 }
 
 int kernrt_cuda_pages_create(kernrt_cuda_ctx *ctx, int kind, size_t n_layers, size_t n_heads, size_t n_kv_heads,

@@ -24,6 +24,30 @@ def context(n):
         del os.environ["KERNRT_CUDA_FAIL_MALLOC"]
 
 
+def test_kept_memory_goes_back_to_the_device_when_asked():
+    import torch
+
+    with kernrt_b200.CudaBackend(0) as b:
+        b.release_freed()  # nothing kept
+        x = b.upload(np.ones(1000, np.float32))
+        h = b.alloc_bytes(6 << 30)
+        b.synchronize()
+        held = torch.cuda.mem_get_info(0)[0]
+        b.free(h)
+        assert torch.cuda.mem_get_info(0)[0] < held + (1 << 30)  # kept
+        b.release_freed()
+        assert torch.cuda.mem_get_info(0)[0] > held + (5 << 30)
+        assert (b.read(x, 1000) == 1).all()
+        stream, g = torch.cuda.ExternalStream(b.stream()), torch.cuda.CUDAGraph()
+        y = b.alloc(1000)
+        b.synchronize()
+        with torch.cuda.graph(g, stream=stream):
+            b.copy(x, 0, y, 0, 1000)
+            with pytest.raises(KernrtCudaError) as e:
+                b.release_freed()
+        assert e.value.code == kernrt_b200.E_STATE
+
+
 MATRIX = np.arange(64 * 32, dtype=np.float32).reshape(64, 32)
 CALLS = {
     "alloc": lambda b: b.alloc(5000),

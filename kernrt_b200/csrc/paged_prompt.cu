@@ -378,6 +378,37 @@ __device__ __forceinline__ bool loader_or(bool p) {
     return r != 0;
 }
 
+// The rows of a warp whose bits are in `rest` attended again, four at a time: a
+// lane's row has its query at q + at and its values at o + to, the result or, with
+// ml, a part's.
+__device__ __noinline__ void attend_again(const PagesView &p, int layer, int j, const int32_t *table, const float *q,
+                                          float *o, float2 *ml, size_t at, size_t to, int lo, int limit, unsigned rest) {
+    constexpr int R = 4;
+    const int lane = threadIdx.x & 31;
+    while (rest) {
+        const float *qs[R];
+        int his[R], of[R];
+#pragma unroll
+        for (int x = 0; x < R; ++x) {  // (the last again where there are fewer)
+            of[x] = rest ? __ffs((int)rest) - 1 : of[x - 1];
+            rest &= rest - 1;
+            qs[x] = q + __shfl_sync(0xffffffffu, at, of[x]);
+            his[x] = __shfl_sync(0xffffffffu, limit, of[x]);
+        }
+        RowAcc a[R];
+        attend_rows<R>(p, layer, j, table, qs, lo, his, a);
+#pragma unroll
+        for (int x = 0; x < R; ++x) {
+            float *dst = o + __shfl_sync(0xffffffffu, to, of[x]);
+            const float l = ml ? 1.0f : a[x].l;
+#pragma unroll
+            for (int i = 0; i < kHeadMax / 32; ++i)
+                if (lane + 32 * i < p.head) dst[lane + 32 * i] = a[x].o[i] / l;
+            if (ml && lane == of[x]) *ml = make_float2(a[x].m, a[x].l);
+        }
+    }
+}
+
 template <int T>
 struct Tile {  // a number known at compile time
     __device__ __forceinline__ constexpr operator int() const { return T; }
@@ -612,20 +643,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                         dst[d / 2] = make_float4(acc[d].x * f, acc[d].y * f, acc[d + 1].x * f, acc[d + 1].y * f);
                 if (it.n_parts > 1) scratch.ml[part] = make_float2(m, l * 0x1p-14f);
             }
-            unsigned rest = __ballot_sync(0xffffffffu, live && !fine);
-            while (rest) {
-                const int w = __ffs((int)rest) - 1;
-                rest &= rest - 1;
-                const size_t at_w = __shfl_sync(0xffffffffu, at, w), part_w = __shfl_sync(0xffffffffu, part, w);
-                const RowAcc a = attend_row(p, layer, j, table, q + at_w, it.lo, __shfl_sync(0xffffffffu, limit, w));
-#pragma unroll
-                for (int i = 0; i < kHeadMax / 32; ++i) {
-                    const int d = lane + 32 * i;
-                    if (d >= p.head) continue;
-                    if (it.n_parts == 1) out[at_w + d] = a.o[i] / a.l;
-                    else scratch.o[part_w * p.head + d] = a.o[i];
-                }
-                if (it.n_parts > 1 && lane == 0) scratch.ml[part_w] = make_float2(a.m, a.l);
+            const unsigned rest = __ballot_sync(0xffffffffu, live && !fine);
+            if (rest) {
+                const bool whole = it.n_parts == 1;
+                attend_again(p, layer, j, table, q, whole ? out : scratch.o, whole ? nullptr : scratch.ml + part, at,
+                             whole ? at : part * p.head, it.lo, limit, rest);
             }
         }
     } else if (warp < 12) {

@@ -54,6 +54,7 @@
 // the first: tensor 35 %, issue 53 %): the hand-offs between the roles bound it.
 // Not kept at the first: exponentials by polynomial on the FMA units for half or
 // a quarter of them (545, 501 us against 488), in turns (541 against 498).
+#include <cmath>
 #include <cuda_fp16.h>
 
 #include "kernels.cuh"
@@ -417,7 +418,8 @@ struct Tile {  // a number known at compile time
 template <int D, bool F32>
 __global__ void __launch_bounds__(kPromptThreads, 1)
     k_pages_prompt(PagesView p, int layer, const StepSeq *__restrict__ seqs, const AttnItem *__restrict__ items,
-                   AttnScratch scratch, const float *__restrict__ q, float *__restrict__ out, int *err) {
+                   AttnScratch scratch, const float *__restrict__ q, float *__restrict__ out, int *err, float scale,
+                   float top) {
     using S = Shape<D, F32>;
     constexpr int Keys = S::Keys, W = S::Wide;
     extern __shared__ unsigned char raw_smem[];
@@ -562,8 +564,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             const int rem = limit - (it.lo + tile * Keys);  // the tile's keys this row sees
             const bool masked = __any_sync(0xffffffffu, rem < Keys);
             // (the powers of two first: their product is exact, or far out of use)
-            const float ks = kLog2e * rsqrtf((float)p.head) * (down * s_kscale[tile & (kScaleRing - 1)]);
-            again = again || (rem > 0 && !(ks * (float)p.head <= kScoreTop));
+            const float ks = scale * (down * s_kscale[tile & (kScaleRing - 1)]);
+            again = again || (rem > 0 && ks > top);
             float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             // (rolled loops: the roles' code competes for the instruction caches)
 #pragma unroll 1
@@ -909,7 +911,8 @@ cudaError_t launch(const PagesView &p, int layer, const StepSeq *seqs, const Att
         attr_done[dev] = true;
     }
     const cudaError_t e = launch_after(k_pages_prompt<D, F32>, dim3((unsigned)p.kv_heads * (unsigned)n_items),
-                                       kPromptThreads, Shape<D, F32>::Smem, s, p, layer, seqs, items, scratch, q, out, err);
+                                       kPromptThreads, Shape<D, F32>::Smem, s, p, layer, seqs, items, scratch, q, out, err,
+                                       kLog2e / std::sqrt((float)p.head), kScoreTop / (float)p.head);
     if (e != cudaSuccess) return e;
     count_launch();
     return cudaGetLastError();

@@ -31,7 +31,9 @@
 // the row does see, and the row is NaN.  Weights, carried to 2^-39 of the largest,
 // are taken relative to the largest of their row and tile, not of the row so far,
 // and the difference joins the tile's scale: large values further on may count
-// with weights far below it.
+// with weights far below it.  Where the largest weight's own value is zero, or next
+// to it, all that is left may lie below 2^-39: a row whose sums end that far below
+// the tiles' scales is attended again.
 // The marks travel with the tiles' scales (a negative scale of V, an infinite one
 // of K), so that they reach the same rows every time, however far ahead the loader
 // is.  (NaN stays out of the tiles' largest.)
@@ -73,6 +75,10 @@ constexpr int kPromptThreads = 512;
 // 2^14 at most and twice for q and K makes 2^-10 an element of the head before the
 // factor, and 2^-18 (in powers of two) of the score with this one.
 constexpr float kScoreTop = 0x1p-8f;
+// A weight is off by up to 2^-25 (of at most 2^14) below 2^-3, so a tile's sums by
+// 2^-11 a key and 2^-4 in all, times the scale: 2^-16 of a row whose largest sum
+// is this many scales.  Ordinary values: 2^25 and more.
+constexpr float kLost = 0x1p12f;
 constexpr int kScaleRing = 16;  // tiles' scales; the loader is at most 4 tiles ahead
 
 template <int D, bool F32>
@@ -529,6 +535,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         for (int d = 0; d < D / 2; ++d) acc[d] = both(0.0f);
         float m = -INFINITY, l = 0.0f;
         float f = 0.0f;      // the weights' own scale in the last tile, 2^(its maximum - m)
+        float e = 0.0f;      // what acc may be off by, less kLost
         bool again = false;  // the row is attended again in f32
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t o_at = tmem + lanes + (uint32_t)(S::SumAt + (S::Sums == 2 ? t * D : 0));
@@ -537,6 +544,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             if (!__all_sync(0xffffffffu, wait(&o_full[t], (uint32_t)tile & 1u))) return false;
             tc_fence_after();
             const float mark = s_vscale[tile & (kScaleRing - 1)], vs = f * fabsf(mark);
+            e += vs;
             again = again || (mark < 0.0f && limit > it.lo + tile * Keys);
             tmem_each<D, W>(o_at, [&](int c, uint32_t(&v)[W]) {
 #pragma unroll
@@ -587,6 +595,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             if (tile && __any_sync(0xffffffffu, mn > m)) {
                 const float keep = mn == -INFINITY ? 0.0f : ex2(m - mn);
                 l *= keep;
+                e *= keep;
 #pragma unroll
                 for (int d = 0; d < D / 2; ++d) acc[d] = mul2(acc[d], both(keep));
             }
@@ -631,8 +640,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (S::Sums == 2 && ok && mine) ok = flush(mine - 1);
         if (ok) {
             bool fine = isfinite(l);
+            float most = 0.0f;
 #pragma unroll
-            for (int d = 0; d < D / 2; ++d) fine = fine && isfinite(acc[d].x) && isfinite(acc[d].y);
+            for (int d = 0; d < D / 2; ++d) {
+                fine = fine && isfinite(acc[d].x) && isfinite(acc[d].y);
+                most = fmaxf(most, fmaxf(fabsf(acc[d].x), fabsf(acc[d].y)));
+            }
+            fine = fine && most >= e * kLost;
             fine = fine || l != l;  // (a NaN score among the row's own: dividing by l says so)
             fine = fine && !again;
             const size_t part = ((size_t)item * p.kv_heads + j) * kRows + r;
@@ -726,7 +740,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 const bool inf = most == 0x7f800000u;
                 const bool mark = inf || too_wide<F32>(most, least);
                 const float down = down_scale(up);
-                if (is_v(i)) s_vscale[tile_of(i) & (kScaleRing - 1)] = mark ? -down : down;
+                if (is_v(i)) s_vscale[tile_of(i) & (kScaleRing - 1)] = mark ? -down : most ? down : 0.0f;
                 else s_kscale[tile_of(i) & (kScaleRing - 1)] = inf ? INFINITY : down;
             }
             const uint32_t dst =

@@ -175,3 +175,30 @@ def test_small_weights_of_large_values(gpu, kind, level, size):
     data = leveled(10, levels, sizes)
     c, out = attend(gpu, kind, data, *MANY)
     check(c, data, out, [1029, 1030, 1100, 1151, 1290], [0, 9, 63])
+
+
+@KINDS
+@pytest.mark.parametrize("level", [-15, -25, -45], ids=str)
+@pytest.mark.parametrize("size", [0.0, 1e-30], ids=["zero", "tiny"])
+def test_a_key_of_most_weight_whose_value_is_zero(gpu, kind, level, size):
+    """All of the output comes from keys of its tile with weights far below it."""
+    levels, sizes = np.full(1300, -120.0), np.ones(1300)
+    levels[1030], sizes[1030] = 0, size
+    levels[1031:1150] = level
+    data = leveled(11, levels, sizes)
+    c, out = attend(gpu, kind, data, *MANY)
+    check(c, data, out, [1031, 1100, 1149, 1151, 1290], [0, 9, 63])
+    assert not np.isnan(out).any()
+
+
+@KINDS
+def test_values_of_zero(gpu, kind):
+    data = normal(12)
+    data[2][:] = 0
+    c, out = attend(gpu, kind, data)
+    assert (out == 0).all()
+    data = normal(12)
+    data[2][:, 3 * D:4 * D] = 0
+    data[2][:, 7::D] = 0
+    c, out = attend(gpu, kind, data)
+    check(c, data, out, [0, 255, 256, 777, 1099], [0, 6, 7, 15], by_one=False)

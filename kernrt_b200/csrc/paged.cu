@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(256) k_pages_step(PagesView p, const StepSeq *
 // after every 16 tiles (4 for wide f32 heads) the sums go to shared memory, where
 // they are added with rounding (added in registers after every tile, one token of
 // 64 sequences of 100 to 8000 keys, 16 heads of 128, took 207 us instead of 177).
-// Bound by HBM: 131072 keys of 8 kv heads of 128 in bf16 take 93.5 us, 5.7 TB/s.
+// Bound by HBM: 131072 keys of 8 kv heads of 128 in bf16 take 91.5 us, 5.9 TB/s.
 template <int NB>
 struct QFrag {  // [block of 32][half of it]: A of parts 1 and 2, and of part 3
     uint32_t a[NB][2][4], c[NB][2][2];

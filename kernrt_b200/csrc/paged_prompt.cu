@@ -17,26 +17,30 @@
 // tile's largest, and f32 values (as two halves, three products) to 2^-22 of
 // their own or 2^-39 of the tile's largest, whichever is more; query rows
 // likewise, row by row.  The scales return as one factor of the scores and one of
-// the tile's sum.  A score only needs its absolute error small, and the row's and
-// the tile's largest bound it, whether or not they meet in a score that counts: it
-// is below 2^-18 while their product stays below 2^14 (heads of 128; 2^15 for 64).
-// Beyond, the row is attended again by attend_row in f32, over the keys it sees
-// alone.  Values are asked for more, because the tile's largest may stand in a
-// row that is masked or has no weight, or in another column: where some group of
-// neighbours of a row or of a column lies more than 2^16 below the tile's largest
-// and is not zero, the rows that see some of the tile are attended again, too.  (So
-// a value is off by at most 2^-23 of the largest of its neighbours.)  So they are
-// where the tile or their query holds an infinity, and so are rows whose
-// result is not finite, unless their sum of weights is NaN: that takes a NaN score
-// the row does see, and the row is NaN.  Weights, carried to 2^-39 of the largest,
-// are taken relative to the largest of their row and tile, not of the row so far,
-// and the difference joins the tile's scale: large values further on may count
-// with weights far below it.  Where the largest weight's own value is zero, or next
-// to it, all that is left may lie below 2^-39: a row whose sums end that far below
-// the tiles' scales is attended again.
+// the tile's sum.  Weights are taken relative to the largest of their row and tile,
+// not of the row so far, and the difference joins the tile's scale: values far
+// larger in another tile count with weights far smaller.
+//
+// What the halves cannot carry is found here and attended again by attend_rows in
+// f32, row by row, each over the keys it sees alone (20 to 65 times as long):
+// - Scores.  What an element loses beside its row's or its tile's largest is
+//   bounded by the two largest, whether or not they meet in a score that counts:
+//   less than 2^-18 of a score while their product stays below 2^14 (heads of 128;
+//   2^15 for 64).  Rows beyond go again.
+// - Values.  The tile's largest may stand in a row that is masked or has no weight,
+//   or in another column.  Where some group of neighbours of a row or of a column
+//   lies more than 2^16 below it and is not zero, the rows that see some of the tile
+//   go again: no value is off by more than 2^-23 of the largest of its neighbours.
+// - Weights.  Where the largest weight's own value is zero, or next to it, all that
+//   is left may lie below 2^-39: rows whose sums end that far below the tiles'
+//   scales go again.
+// - Infinities in the tile or in the query, and results that are not finite, unless
+//   the sum of weights is NaN: that takes a NaN score the row does see, and the row
+//   is NaN.  (NaN stays out of the tiles' largest.)
 // The marks travel with the tiles' scales (a negative scale of V, an infinite one
 // of K), so that they reach the same rows every time, however far ahead the loader
-// is.  (NaN stays out of the tiles' largest.)
+// is.
+//
 // The tensor cores add into an f32 accumulator with truncation: measured
 // relative error 1.1e-9 per K (9e-6 at K = 8192, always toward zero), so
 // a tile's sum of V is taken out of TMEM after every 64 or 128 keys and added in
@@ -50,12 +54,14 @@
 // registers, a ring of tiles K0 K1 V0 K2 V1 ..  Warp 12: one thread issues the MMAs.
 // Every wait is bounded: one that runs out sets ERR_TIMEOUT and the roles stop.
 //
-// Measured (causal, bf16 pages, 8 kv heads, 8192 tokens): 24 heads of 64 489 us,
-// 16 heads of 128 484 us (568 TFLOP/s without counting the halves twice); f32
-// pages, 32 heads of 64, 4096 tokens: 235 us.  No pipe is near full (at 4096 of
-// the first: tensor 35 %, issue 53 %): the hand-offs between the roles bound it.
-// Not kept at the first: exponentials by polynomial on the FMA units for half or
-// a quarter of them (545, 501 us against 488), in turns (541 against 498).
+// Measured (causal, bf16 pages, 8 kv heads, 8192 tokens, back to back): 24 heads of
+// 64 501 us, 16 heads of 128 482 us (570 TFLOP/s without counting the halves
+// twice); f32 pages, 32 heads of 64, 4096 tokens: 248 us.  No pipe is near full (at
+// 4096 of the first: tensor 34 %, exponentials 35 %, issue slots 53 %): the latency
+// of a row's chain from scores to weights to sums bounds it, two warps a scheduler.
+// Not kept at an earlier step of the first: exponentials by polynomial on the FMA
+// units for half or a quarter of them (545, 501 us against 488), in turns (541
+// against 498).
 #include <cmath>
 #include <cuda_fp16.h>
 

@@ -96,6 +96,7 @@ struct Shape {
     static constexpr int Slots = D == 64 ? (F32 ? 4 : 6) : 3;
     static constexpr int QTile = 2 * (D / 64) * 128 * 128;  // both halves of 128 rows
     static constexpr size_t Smem = 2 * (size_t)QTile + (size_t)Slots * Slot + 1024;
+    static constexpr int Step = 1024 / D;  // rows that the loader's threads take at once
     static constexpr int Wide = D == 64 ? 32 : 16;  // columns a softmax thread takes at a time
     // TMEM columns: three buffers of scores / weights, which the two query
     // tiles take in turn, and the sums of V of both tiles or, where they do not
@@ -321,7 +322,8 @@ __device__ __forceinline__ uint32_t min_u16x2(uint32_t a, uint32_t b) {
 // How far values may spread, in powers of two: the largest of a few neighbours
 // below their tile's largest.  The neighbours are eight elements of a row (of bf16
 // the four even or the four odd ones), and a thread's N rows of a column.  (Of a
-// single row an element is no group: an ordinary one is small now and then.)
+// single row an element is no group: an ordinary one is small now and then.
+// Sequences too short for two rows a thread have a check of their own, short_wide.)
 constexpr int kSpread = 16;
 // The largest magnitude (as f32 bits) of a thread's share of a tile, eight elements
 // of each of N rows, and the least of its rows' largest, less one step of their
@@ -389,6 +391,31 @@ __device__ __forceinline__ bool loader_or(bool p) {
         : "r"((uint32_t)p)
         : "memory");
     return r != 0;
+}
+
+// Whether the columns of the values of a sequence of `n` keys, at most 32, spread
+// too far, by a whole warp.
+template <bool F32>
+__device__ __forceinline__ bool short_wide_of(const PagesView &p, int layer, int j, const int32_t *table, int n) {
+    const int page_mask = (1 << p.page_shift) - 1;
+    const size_t first = page_elem(p, layer, 1, table[0], j);
+    const size_t second = n > page_mask + 1 ? page_elem(p, layer, 1, table[1], j) : first;
+    uint32_t most = 0, least = 0xffffffffu;
+    for (int d = threadIdx.x & 31; d < p.head; d += 32) {
+        float m = 0.0f;
+#pragma unroll 8
+        for (int t = 0; t < n; ++t) {
+            const size_t e = (t > page_mask ? second : first) + (size_t)(t & page_mask) * p.head + d;
+            if constexpr (F32) m = fmaxf(m, fabsf(static_cast<const float *>(p.kv)[e]));
+            else m = fmaxf(m, fabsf(__bfloat162float(static_cast<const __nv_bfloat16 *>(p.kv)[e])));
+        }
+        most = max(most, __float_as_uint(m));
+        least = min(least, __float_as_uint(m) - 1);
+    }
+    return too_wide<true>(__reduce_max_sync(0xffffffffu, most), __reduce_min_sync(0xffffffffu, least));
+}
+__device__ __noinline__ bool short_wide(const PagesView &p, int layer, int j, const int32_t *table, int n) {
+    return p.f32 ? short_wide_of<true>(p, layer, j, table, n) : short_wide_of<false>(p, layer, j, table, n);
 }
 
 // The rows of a warp whose bits are in `rest` attended again, four at a time: a
@@ -655,6 +682,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             fine = fine && most >= e * kLost;
             fine = fine || l != l;  // (a NaN score among the row's own: dividing by l says so)
             fine = fine && !again;
+            if (it.lo == 0 && it.hi < 2 * S::Step && short_wide(p, layer, j, table, it.hi)) fine = false;
             const size_t part = ((size_t)item * p.kv_heads + j) * kRows + r;
             if (live && fine) {
                 const float f = it.n_parts == 1 ? 1.0f / l : 0x1p-14f;
@@ -675,7 +703,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     } else if (warp < 12) {
         // ---- the loader: tiles K0 K1 V0 K2 V1 .. V(n-1) ---------------------------------
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        constexpr int PerRow = D / 8, Step = 128 / PerRow;  // eight-element chunks of a row, rows of a step
+        constexpr int PerRow = D / 8, Step = S::Step;  // eight-element chunks of a row, rows of a step
         constexpr int Loads = Keys / Step;
         const int tid = threadIdx.x - 256, chunk = tid % PerRow, row = tid / PerRow;
         constexpr uint32_t Size = F32 ? 4 : 2;
@@ -720,12 +748,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             const int next = min(i + 1, 2 * n - 1);
             const size_t place_next = places(tile_of(min(i + 2, 2 * n - 1)));
             // the tile's largest magnitude and, of V, the smallest of its groups'
-            // (columns where this thread has rows, not one, or the first tile is all)
+            // (columns where this thread has rows, not one)
             uint32_t most, least;
             rows_spread<F32, Loads>(v, most, least);
             if (is_v(i)) {
-                const int at = tile_of(i);
-                if (room_of(at) > Step || it.lo + at == 0) least = min(least, columns_spread<F32, Loads>(v));
+                if (room_of(tile_of(i)) > Step) least = min(least, columns_spread<F32, Loads>(v));
                 least = __reduce_min_sync(0xffffffffu, least);
             }
             most = __reduce_max_sync(0xffffffffu, most);

@@ -30,16 +30,17 @@ def check(c, data, out, rows, heads, by_one=True):
     """Some rows of a first step of one sequence."""
     q, k, v = data
     n = len(q)
-    q = q.astype(np.float64).reshape(n, c.heads, D)
-    k, v = (rounded(x, c.kind).reshape(n, c.kv_heads, D) for x in (k, v))
+    d = c.head
+    q = q.astype(np.float64).reshape(n, c.heads, d)
+    k, v = (rounded(x, c.kind).reshape(n, c.kv_heads, d) for x in (k, v))
     for r in rows:
         m = r + 1
         adds = (m if by_one else m / 64) + 16
         rest = 2 * 2.0 ** -18 + 3 * 2.0 ** -22 + 32 * 2.0 ** -23 + adds * 2.0 ** -24
         for h in heads:
             kj, vj = k[:m, h * c.kv_heads // c.heads], v[:m, h * c.kv_heads // c.heads]
-            x = kj @ q[r, h] / math.sqrt(D)
-            dx = np.abs(kj) @ np.abs(q[r, h]) / math.sqrt(D) * (3 * 2.0 ** -22 + D * 2.0 ** -23) + 2.0 ** -18
+            x = kj @ q[r, h] / math.sqrt(d)
+            dx = np.abs(kj) @ np.abs(q[r, h]) / math.sqrt(d) * (3 * 2.0 ** -22 + d * 2.0 ** -23) + 2.0 ** -18
             p = np.exp(x - x.max())
             p /= p.sum()
             o = p @ vj
@@ -202,3 +203,23 @@ def test_values_of_zero(gpu, kind):
     data[2][:, 7::D] = 0
     c, out = attend(gpu, kind, data)
     check(c, data, out, [0, 255, 256, 777, 1099], [0, 6, 7, 15], by_one=False)
+
+
+@KINDS
+@pytest.mark.parametrize("head", [64, 128])
+def test_short_sequences_among_prompts(gpu, kind, head):
+    """Sequences of a few keys packed with a prompt: large columns, large values in
+    later rows, a large key; and ordinary ones, which no check sends the long way."""
+    rng = np.random.default_rng(13)
+    lens = [1500, 1, 2, 7, 9, 15, 17, 31, 32, 33, 40]
+    starts = np.cumsum([0] + lens[:-1])
+    total = sum(lens)
+    q, k, v = (rng.standard_normal((total, w * head)).astype(np.float32) for w in (32, 8, 8))
+    v[lens[0]:, 2::8] *= 1e12
+    for a, n in zip(starts, lens):
+        k[a + n // 2 + 1:a + n, 9::head] *= 1e12
+    with Pair(gpu, kind, 32, 8, head, 16, total // 16 + 20, len(lens), 1500) as c:
+        seqs = [c.open() for _ in lens]
+        out = c.step(seqs, lens, [(q, k, v)], check=False)[0]
+        for a, n in zip(starts, lens):
+            check(c, [x[a:a + n] for x in (q, k, v)], out[a:a + n], sorted({0, n // 2, n - 1}), [0, 13, 31])

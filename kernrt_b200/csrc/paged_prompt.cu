@@ -569,7 +569,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         float m = -INFINITY, l = 0.0f;
         float f = 0.0f;      // the weights' own scale in the last tile, 2^(its maximum - m)
         float e = 0.0f;      // what acc may be off by, less kLost
-        bool again = false;  // the row is attended again in f32
+        // the row is attended again in f32
+        bool again = it.lo == 0 && it.hi < 2 * S::Step && short_wide(p, layer, j, table, it.hi);
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t o_at = tmem + lanes + (uint32_t)(S::SumAt + (S::Sums == 2 ? t * D : 0));
         // the sum of V over a key tile, once it is there, into the registers
@@ -682,7 +683,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             fine = fine && most >= e * kLost;
             fine = fine || l != l;  // (a NaN score among the row's own: dividing by l says so)
             fine = fine && !again;
-            if (it.lo == 0 && it.hi < 2 * S::Step && short_wide(p, layer, j, table, it.hi)) fine = false;
             const size_t part = ((size_t)item * p.kv_heads + j) * kRows + r;
             if (live && fine) {
                 const float f = it.n_parts == 1 ? 1.0f / l : 0x1p-14f;

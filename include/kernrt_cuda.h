@@ -473,10 +473,11 @@ int kernrt_cuda_pages_write(kernrt_cuda_ctx *ctx, kernrt_pages pages, size_t lay
 /* out[r, h] = softmax(q[r, h] . K / sqrt(head_size)) V for the step's rows, f32
  * [rows, n_heads * head_size], over positions 0 .. the row's own; head h reads
  * kv head h / (n_heads / n_kv_heads).  q != out.  Scores are f32: a row with one past
- * its range is NaN.  Rows of many-row calls whose operands are too large or spread
- * too far for the tensor cores' 16-bit halves (a product of magnitudes of q and k
- * from about 2^14, values more than 2^16 below their neighbours within 64 or 128
- * keys, infinities) take a slower path in f32, 20 to 65 times as long. */
+ * its range is NaN.  In calls of many rows, those whose operands the tensor cores'
+ * 16-bit halves cannot carry take a slower path in f32, 20 to 65 times as long:
+ * infinities; a product of the largest magnitudes of a query and of 64 or 128
+ * neighbouring keys from about 2^14 on; among as many values, rows or columns
+ * more than 2^16 below the largest. */
 int kernrt_cuda_pages_attention(kernrt_cuda_ctx *ctx, kernrt_pages pages, size_t layer, kernrt_buf q, kernrt_buf out);
 
 /* --- Log probabilities of given tokens -------------------------------------------

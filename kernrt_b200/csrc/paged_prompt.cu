@@ -55,8 +55,9 @@
 // Every wait is bounded: one that runs out sets ERR_TIMEOUT and the roles stop.
 //
 // Measured (causal, bf16 pages, 8 kv heads, 8192 tokens, back to back): 24 heads of
-// 64 501 us, 16 heads of 128 482 us (570 TFLOP/s without counting the halves
-// twice); f32 pages, 32 heads of 64, 4096 tokens: 248 us.  No pipe is near full (at
+// 64 503 us, 16 heads of 128 490 us (561 TFLOP/s without counting the halves
+// twice); f32 pages, 32 heads of 64, 4096 tokens: 250 us; the checks of what the
+// halves carry cost 1 to 3 % of it.  No pipe is near full (at
 // 4096 of the first: tensor 34 %, exponentials 35 %, issue slots 53 %): the latency
 // of a row's chain from scores to weights to sums bounds it, two warps a scheduler.
 // Not kept at an earlier step of the first: exponentials by polynomial on the FMA
